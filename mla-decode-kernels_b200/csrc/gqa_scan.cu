@@ -24,6 +24,7 @@
 // sum(l_i f_i) (kernels/gqa_decode/v2_splitkv.cu:97-107).
 #include <math.h>
 
+#include "gqa_balance.cuh"
 #include "gqa_internal.h"
 #include "gqa_ptx.cuh"
 
@@ -74,24 +75,6 @@ struct Seg {
   int nparts;      // number of segments the row was cut into
   long long cfirst;  // BALANCED: index of the first CTA that holds this row
 };
-
-// BALANCED ranges: the T stages of all rows, in row order, are cut into E =
-// min(grid, T / 2) ranges with proportional boundaries [c T / E, (c+1) T / E)
-// - sizes differ by at most one stage, and every range holds at least two
-// stages so that no row is cut into single-stage parts.  CTAs c >= E idle.
-__device__ __forceinline__ long long range_parts(long long T, long long grid) {
-  return max(1LL, min(grid, T / 2));
-}
-
-__device__ __forceinline__ long long range_start(long long c, long long T, long long E) {
-  return c >= E ? T : c * T / E;
-}
-
-// The range that holds stage g (0 <= g < T): the largest c with
-// c T / E <= g, i.e. c T < (g + 1) E.
-__device__ __forceinline__ long long range_owner(long long g, long long T, long long E) {
-  return ((g + 1) * E - 1) / T;
-}
 
 struct SegIter {
   // FIXED
@@ -160,65 +143,6 @@ __device__ __forceinline__ bool iter_next(SegIter& it, const ScanParams& p, long
     return true;
   }
   return false;
-}
-
-// Block-wide start of the CTA's range in the BALANCED schedule.  Every
-// thread takes part; afterwards sh_* hold the range and its first request.
-__device__ __forceinline__ void balanced_start(const ScanParams& p, long long cap, long long* sh_warp,
-                               long long* sh_info) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int nthr = blockDim.x, nwarps = nthr >> 5;
-  const int chunk = (p.B + nthr - 1) / nthr;
-  const int blo = min(p.B, tid * chunk), bhi = min(p.B, blo + chunk);
-  long long local = 0;
-  for (int b = blo; b < bhi; ++b)
-    local += (req_len(p, b, cap) + kStageTokens - 1) / kStageTokens;
-  long long x = local;
-  #pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const long long y = __shfl_up_sync(kFull, x, off);
-    if (lane >= off) x += y;
-  }
-  if (lane == 31) sh_warp[warp] = x;
-  __syncthreads();
-  if (warp == 0) {
-    long long t = lane < nwarps ? sh_warp[lane] : 0;
-    #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const long long y = __shfl_up_sync(kFull, t, off);
-      if (lane >= off) t += y;
-    }
-    if (lane < nwarps) sh_warp[lane] = t;
-  }
-  __syncthreads();
-  const long long excl = x - local + (warp > 0 ? sh_warp[warp - 1] : 0);
-  const long long total = sh_warp[nwarps - 1];
-  const long long T = total * p.NHG;
-  const long long E = range_parts(T, gridDim.x);
-  const long long g0 = range_start(blockIdx.x, T, E);
-  const long long g1 = range_start(blockIdx.x + 1LL, T, E);
-  if (tid == 0) {
-    sh_info[0] = g0;
-    sh_info[1] = g1;
-    sh_info[2] = E;
-    sh_info[3] = 0;  // first request
-    sh_info[4] = 0;  // stages before it
-    sh_info[5] = T;
-  }
-  __syncthreads();
-  if (g0 < g1 && g0 >= excl * p.NHG && g0 < (excl + local) * p.NHG) {
-    long long P = excl;
-    for (int b = blo; b < bhi; ++b) {
-      const long long L = (req_len(p, b, cap) + kStageTokens - 1) / kStageTokens;
-      if (g0 < (P + L) * p.NHG) {
-        sh_info[3] = b;
-        sh_info[4] = P;
-        break;
-      }
-      P += L;
-    }
-  }
-  __syncthreads();
 }
 
 __device__ __forceinline__ void store_bf16x4(__nv_bfloat16* dst, float a, float b, float c,
@@ -293,7 +217,12 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
     }
     __syncthreads();
   } else if (p.schedule == kBalanced) {
-    balanced_start(p, cap, sh_warp, sh_info);  // contains __syncthreads
+    balanced_start(
+        p.B, p.NHG,
+        [&](int b) -> long long {
+          return (req_len(p, b, cap) + kStageTokens - 1) / kStageTokens;
+        },
+        sh_warp, sh_info);  // contains __syncthreads
   } else {
     __syncthreads();
   }

@@ -26,9 +26,11 @@ EXT_NAME = "gqa_decode_ext"
 EXT_PATH = os.path.join(BUILD_DIR, EXT_NAME + ".so")
 
 CU_SOURCES = ["gqa_scan.cu", "gqa_simt.cu", "gqa_api.cu", "gqa_cxx_abi.cu", "gqa_noalloc.cu",
-              "mla_decode.cu", "dsa_decode.cu"]
-CU_HEADERS = ["gqa_internal.h", "gqa_ptx.cuh", "gqa_merge.cuh", "umma_ptx.cuh", "device_once.h"]
-PUBLIC_HEADERS = ["gqa_decode.h", "mla_decode.h", "dsa_decode.h"]
+              "mla_decode.cu", "dsa_decode.cu", "kv_append.cu", "kv4_decode.cu"]
+CU_HEADERS = ["gqa_internal.h", "gqa_ptx.cuh", "gqa_merge.cuh", "gqa_balance.cuh", "umma_ptx.cuh",
+              "device_once.h", "kv_tokens.cuh", "kv4_tile.cuh"]
+PUBLIC_HEADERS = ["gqa_decode.h", "mla_decode.h", "dsa_decode.h", "kv_append.h", "kv4_decode.h"]
+EXT_SOURCES = ["gqa_decode_ext.cpp", "kv_cache_ext.cpp"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -77,9 +79,9 @@ def preload_lib():
 
 
 def build_ext(force=False, verbose=False):
-    """Compile python/gqa_decode_ext.cpp against the C ABI into _build/."""
-    src = os.path.join(PY_DIR, "gqa_decode_ext.cpp")
-    deps = [src, LIB_PATH] + [os.path.join(INCLUDE_DIR, h) for h in PUBLIC_HEADERS]
+    """Compile the binding's sources against the C ABI into _build/."""
+    srcs = [os.path.join(PY_DIR, s) for s in EXT_SOURCES]
+    deps = srcs + [LIB_PATH] + [os.path.join(INCLUDE_DIR, h) for h in PUBLIC_HEADERS]
     if not force and not _newer(EXT_PATH, deps):
         return EXT_PATH
     preload_lib()
@@ -88,7 +90,7 @@ def build_ext(force=False, verbose=False):
     os.makedirs(BUILD_DIR, exist_ok=True)
     load(
         name=EXT_NAME,
-        sources=[src],
+        sources=srcs,
         build_directory=BUILD_DIR,
         extra_include_paths=[INCLUDE_DIR],
         extra_cflags=["-O3"],

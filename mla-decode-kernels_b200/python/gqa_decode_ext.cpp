@@ -17,6 +17,9 @@
 #include "mla_decode.h"
 #include "dsa_decode.h"
 
+// The cache-append and 4-bit-cache functions (kv_cache_ext.cpp).
+void bind_kv_cache(pybind11::module_& m);
+
 namespace {
 
 struct GqaDims {
@@ -761,6 +764,7 @@ torch::Tensor dsa_gather(torch::Tensor kv_cache, torch::Tensor block_table, torc
 int64_t dsa_get_status(bool clear) { return dsa_decode_get_status(clear ? 1 : 0); }
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+  bind_kv_cache(m);
   m.def("mla_decode", &mla_decode, "MLA latent-cache paged decode (tcgen05)", py::arg("q"),
         py::arg("kv_cache"), py::arg("block_table"), py::arg("seq_lens"),
         py::arg("softmax_scale"), py::arg("causal"), py::arg("num_splits"), py::arg("workspace"));
