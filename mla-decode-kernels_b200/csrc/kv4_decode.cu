@@ -6,21 +6,30 @@
 //     q . k_t = sum_y s_ty (sum_d q_d (n_td - 8)) + sum_y c_ty Q_y,
 //     out_d   = sum_t (p_t s_ty) (n_td - 8) + sum_t p_t c_ty,
 // so neither scale nor centre is ever applied to a code: K's products with
-// the raw codes are summed per group on the tensor cores and scaled after,
-// V's scales are folded into the softmax weights of each group, and both
-// centre terms are one small tensor-core product per tile.  A code becomes
-// bf16 128 + n by one and-or on its word; K removes the offset through the
-// accumulator's start value -136 Q_y, V by one packed subtraction (exact),
-// since over a long sequence the sum of 136 p s would swamp fp32.
+// the codes are summed per group on the tensor cores and scaled after, V's
+// scales are folded into the softmax weights of each group, and both centre
+// terms are one small tensor-core product per tile.
+//   * K: a masked nibble is the fp16 subnormal n 2^-24 or 16 n 2^-24 as it
+//     stands.  q enters in fp16, divided by a power of two per head so that
+//     its largest element is in [1, 2) (and by 16 more where it meets 16 n);
+//     the accumulator starts at -8 Q_y.  A q element below 2^-17 of its
+//     head's largest loses bits there, 2^-25 of that largest at most.
+//   * V: the nibble becomes 1024 + n or 1024 + 16 n in fp16 by one and-or,
+//     then n - 8 by one packed operation, exactly.  (Codes left positive
+//     would pile up a sum that the centre term takes away again: over a long
+//     context fp32 loses the difference.)  The weights p_t s_ty are rounded
+//     to fp16, 2^-11 instead of bf16's 2^-8.
+// The softmax reference M of a head is no running maximum but any value that
+// keeps the fp16 weights in range: it is set so that the largest p s is 2^9
+// and moves only when one passes 2^15, so the common step takes no maximum
+// and rescales nothing.
 //
-// CTA layout (one persistent CTA per SM, the balanced schedule of
-// gqa_balance.cuh, cut rows merged by the cut-row merge kernel):
-//   * the last warp copies tiles (cp.async.bulk, one per 16-token tile and
-//     row of HG kv heads: contiguous in the cache) into a ring whose slots
-//     hold K or V of 2 TS tiles;
-//   * HG x NT x TS consumer warps: kv head, 8 of its q heads, and every
-//     TS-th pair of tiles.  The TS warps of a head keep their own softmax
-//     state and meet in shared memory at the end of a segment.
+// Layout (one persistent CTA per SM, the balanced schedule of
+// gqa_balance.cuh, cut rows merged by the cut-row merge kernel): HG x NT x TS
+// = up to 16 warps: kv head, 8 of its q heads, and every TS-th pair of tiles.
+// Each warp copies its own tiles (cp.async.bulk, one per tile) into its own
+// ring and refills a slot as soon as it has read it, so no warp waits for
+// another until the TS warps of a head meet at the end of a segment.
 #include <math.h>
 
 #include <algorithm>
@@ -43,18 +52,20 @@ __device__ int g_kv4_status;
 namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
-constexpr int kMaxWarps = 16;                // consumer warps
-constexpr int kMaxSlots = 16;
+constexpr int kMaxWarps = 16;
+constexpr int kMaxUnits = 4;                 // units (pairs of tiles) in a warp's ring
 constexpr int kSmemLimit = 227 * 1024;
-constexpr int kStateWords = 36;              // floats per lane of a warp's softmax state
-constexpr int kStateBytes = kStateWords * 32 * 4;
+constexpr int kSmemStatic = 3 * 1024;        // bound of the kernel's static shared memory
+constexpr int kPassWords = 8;                // floats per lane handed over at once at a meeting
+constexpr float kNoRef = -1e30f;             // M before the first token
 
 __device__ __forceinline__ void raise_status(int bits) { atomicOr(&g_kv4_status, bits); }
 
 // How a launch maps to warps and shared memory (no device state).
 struct Plan {
-  int G, NT, HG, NHG, TS, ncw;
-  int slot_tiles, slot_bytes, nslots, smem;
+  int G, NT, HG, NHG, TS, warps;
+  int units;  // ring depth
+  int smem;
 };
 
 struct DecodeParams {
@@ -98,19 +109,46 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-// Codes j and j + 4 of a word as the bf16 pair (128 + n, 128 + n'): exact,
-// bf16 has 7 fraction bits and 128's last one stands for 1.
-__device__ __forceinline__ uint32_t code_pair(uint32_t w, int j) {
+// K: codes j and j + 4 (j even), or 16 times codes j + 1 and j + 5, of a word
+// shifted by 4 j, in units of 2^-24.
+__device__ __forceinline__ uint32_t low_codes(uint32_t w) { return w & 0x000f000fu; }
+__device__ __forceinline__ uint32_t high_codes(uint32_t w) { return w & 0x00f000f0u; }
+
+// V: the same codes as n - 8 in fp16.  1024 + n and 1024 + 16 n are exact
+// (fp16 counts in ones from 1024 on), and so is what follows.
+__device__ __forceinline__ uint32_t low_centred(uint32_t w) {
   uint32_t r;
-  asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(r) : "r"(w >> (4 * j)));  // (a & b) | c
+  asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(r) : "r"(w));
+  asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(r) : "r"(0x64086408u));  // - 1032
+  return r;
+}
+__device__ __forceinline__ uint32_t high_centred(uint32_t w) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(r) : "r"(w));
+  asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(r) : "r"(0x2c002c00u), "r"(0xd480d480u));  // / 16 - 72
   return r;
 }
 
-// (128 + n) - 136 = n - 8, exact in bf16.
-__device__ __forceinline__ uint32_t centred(uint32_t pair) {
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   uint32_t r;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(pair), "r"(0x43084308u));
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
+}
+
+__device__ __forceinline__ uint32_t max_half2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// D = A(16x16, row) * B(16x8, col) + D, fp16 inputs, fp32 accumulators.
+__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                              uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // The NG bf16 scales of one token as floats.
@@ -133,14 +171,15 @@ __device__ __forceinline__ void load_scales(uint32_t a, float (&s)[NG]) {
 }
 
 struct Seg {
-  int b, hg, row, S, s0, s1, nparts, slot;
+  int b, hg, row, S, s0, s1, nparts;
   long long cfirst;
 };
 
 // The CTA's share of the balanced schedule, as segments (one row, a range of
-// its tiles).
+// its tiles).  Every warp keeps two in shared memory, one ahead of the other:
+// for the copies and for the tiles it works on.
 struct Walk {
-  long long g, g_end, T, E, row0;
+  long long g, g_end, row0;
   int b, hg, S, L;
 };
 
@@ -150,11 +189,16 @@ __device__ __forceinline__ int req_len(const DecodeParams& p, int b) {
   return s < 0 ? 0 : static_cast<int>(min(static_cast<long long>(s), cap));
 }
 
-__device__ __forceinline__ int req_tiles(const DecodeParams& p, int b) {
-  return static_cast<int>((static_cast<long long>(req_len(p, b)) + kTileTokens - 1) / kTileTokens);
+__device__ __forceinline__ int tiles_of(int len) {
+  return static_cast<int>((static_cast<long long>(len) + kTileTokens - 1) / kTileTokens);
 }
 
-__device__ __forceinline__ bool next_seg(Walk& w, const DecodeParams& p, Seg& s) {
+// The next segment of the walk; row_start = its row's first tile in the
+// schedule's order.  Every lane runs it on the same words.
+__device__ __forceinline__ bool next_seg(Walk* wp, const DecodeParams& p, Seg& s,
+                                         long long& row_start) {
+  Walk w = *wp;
+  bool found = false;
   while (w.g < w.g_end) {
     const long long rs = w.row0 + static_cast<long long>(w.hg) * w.L, re = rs + w.L;
     if (w.g >= re) {
@@ -163,10 +207,10 @@ __device__ __forceinline__ bool next_seg(Walk& w, const DecodeParams& p, Seg& s)
         w.row0 += static_cast<long long>(p.pl.NHG) * w.L;
         if (++w.b >= p.B) {
           w.g = w.g_end;
-          return false;
+          break;
         }
         w.S = req_len(p, w.b);
-        w.L = req_tiles(p, w.b);
+        w.L = tiles_of(w.S);
       }
       continue;
     }
@@ -177,156 +221,156 @@ __device__ __forceinline__ bool next_seg(Walk& w, const DecodeParams& p, Seg& s)
     s.S = w.S;
     s.s0 = static_cast<int>(w.g - rs);
     s.s1 = static_cast<int>(e - rs);
-    s.cfirst = range_owner(rs, w.T, w.E);
-    s.nparts = static_cast<int>(range_owner(re - 1, w.T, w.E) - s.cfirst + 1);
-    s.slot = static_cast<int>(blockIdx.x) + s.row;
+    row_start = rs;
     w.g = e;
-    return true;
+    found = true;
+    break;
   }
-  return false;
+  __syncwarp();
+  *wp = w;
+  __syncwarp();
+  return found;
 }
 
 __device__ __forceinline__ void group_barrier(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
-// A warp's softmax state: lane (g, t) holds heads 2 t and 2 t + 1 (n = 0, 1),
-// dims 32 y + 4 g + 2 u + v in acc[2 y + u][2 v + n].
+// Units (pairs of tiles) of a segment of n tiles that warp ts of TS takes:
+// units ts, ts + TS, ...
+__device__ __forceinline__ int my_units(int n, int ts, int TS) {
+  const int units = (n + 1) / 2;
+  return ts < units ? (units - ts + TS - 1) / TS : 0;
+}
+
+// The copies of one warp: the physical tiles of its units, in order, across
+// segments.  Lane i holds the tile of unit first + i / 2, i % 2 of its pair;
+// the next 16 units' block ids are loaded while these are used.
+struct Copier {
+  const int* table;  // the segment's row of the block table
+  int n, s0, hg;     // tiles of the segment, its first tile, its kv-head group
+  int unit, units;   // next unit of this warp, and how many there are
+  uint32_t cur, nxt; // physical tiles (block * tiles per block + place in it)
+
+  __device__ __forceinline__ uint32_t look_up(const DecodeParams& p, int first, int ts) const {
+    const int lane = threadIdx.x & 31;
+    const int u = first + lane / 2;
+    const int tile = 2 * (u * p.pl.TS + ts) + (lane & 1);
+    if (u >= units || tile >= n) return 0;
+    const int lb = (s0 + tile) / p.tiles_per_block, sub = s0 + tile - lb * p.tiles_per_block;
+    int page = ld_nc_s32(table + lb);
+    if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_blocks)) {
+      raise_status(kStatusBadPage);
+      page = 0;
+    }
+    return static_cast<uint32_t>(page) * static_cast<uint32_t>(p.tiles_per_block) + sub;
+  }
+
+  // Tiles of the next unit (1 or 2; 0: no more), each lane's parity's tile in
+  // `tile`.
+  __device__ __forceinline__ int next(const DecodeParams& p, Walk* walk, int ts, uint32_t& tile) {
+    while (unit == units) {
+      Seg s;
+      long long rs;
+      if (!next_seg(walk, p, s, rs)) return 0;
+      table = p.block_table + static_cast<size_t>(s.b) * p.max_blocks;
+      n = s.s1 - s.s0;
+      s0 = s.s0;
+      hg = s.hg;
+      unit = 0;
+      units = my_units(n, ts, p.pl.TS);
+      cur = look_up(p, 0, ts);
+      nxt = look_up(p, 16, ts);
+    }
+    const int i = unit & 15;
+    if (i == 0 && unit > 0) {
+      cur = nxt;
+      nxt = look_up(p, unit + 16, ts);
+    }
+    tile = __shfl_sync(kFull, cur, 2 * i + (threadIdx.x & 1));
+    const int c = min(2, n - 2 * (unit * p.pl.TS + ts));
+    ++unit;
+    return c;
+  }
+};
+
+// A warp's softmax state: lane (g, t) holds heads 2 t and 2 t + 1 (n = 0, 1):
+// the reference M, the weights' sum l and dims 32 y + 4 g + 2 u + v in
+// acc[2 y + u][2 v + n].
 struct State {
   float m[2], l[2];
   float acc[8][4];
 };
 
-__device__ __forceinline__ void merge_state(State& a, const float* other, int lane) {
-  #pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    const float mo = other[n * 32 + lane], lo = other[(2 + n) * 32 + lane];
-    const float m = fmaxf(a.m[n], mo);
-    const float fa = a.m[n] == -INFINITY ? 0.f : exp2_approx(a.m[n] - m);
-    const float fo = mo == -INFINITY ? 0.f : exp2_approx(mo - m);
-    a.m[n] = m;
-    a.l[n] = a.l[n] * fa + lo * fo;
-    #pragma unroll
-    for (int mt = 0; mt < 8; ++mt) {
-      a.acc[mt][n] = a.acc[mt][n] * fa + other[(4 + 4 * mt + n) * 32 + lane] * fo;
-      a.acc[mt][2 + n] = a.acc[mt][2 + n] * fa + other[(4 + 4 * mt + 2 + n) * 32 + lane] * fo;
-    }
-  }
-}
-
-__device__ __forceinline__ void put_state(const State& a, float* dst, int lane) {
-  #pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    dst[n * 32 + lane] = a.m[n];
-    dst[(2 + n) * 32 + lane] = a.l[n];
-  }
-  #pragma unroll
-  for (int mt = 0; mt < 8; ++mt)
-    #pragma unroll
-    for (int i = 0; i < 4; ++i) dst[(4 + 4 * mt + i) * 32 + lane] = a.acc[mt][i];
-}
-
 }  // namespace
 
 template <int NG>
-__global__ void __launch_bounds__((kMaxWarps + 1) * 32, 1)
+__global__ void __launch_bounds__(kMaxWarps * 32, 1)
     kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
   constexpr int kGroup = 128 / NG, kTile = tile_bytes(kGroup);
-  constexpr float kThreshold = 8.f;  // log2 units a score may pass the running maximum by
+  constexpr uint32_t kUnit = 2 * kTile;  // K (or V) of a unit
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ long long sh_warp[32];
   __shared__ long long sh_info[8];
-  __shared__ __align__(8) unsigned long long sh_bar[2 * kMaxSlots];
+  __shared__ __align__(8) unsigned long long sh_bar[kMaxWarps][2][kMaxUnits];
+  __shared__ Walk sh_walk[kMaxWarps][2];
 
   const Plan& pl = p.pl;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t ring = smem_u32(smem);
-  const uint32_t full = smem_u32(sh_bar), empty = full + 8u * kMaxSlots;
+  const int g = lane >> 2, t = lane & 3;
+  const int team = warp / pl.TS, ts = warp - team * pl.TS;  // team = (kv head, q-head tile)
+  const int hl = team / pl.NT, j0 = (team - hl * pl.NT) * 8;
+  const int cnt = min(8, pl.G - j0);
+  float* const scratch = reinterpret_cast<float*>(smem + pl.warps * pl.units * 2 * kUnit) +
+                         static_cast<size_t>(team) * (pl.TS / 2) * kPassWords * 32;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (threadIdx.x == 0) {
-    for (int i = 0; i < pl.nslots; ++i) {
-      mbar_init(full + 8 * i, 1);
-      mbar_init(empty + 8 * i, pl.ncw);
+  if (lane == 0) {
+    for (int i = 0; i < pl.units; ++i) {
+      mbar_init(smem_u32(&sh_bar[warp][0][i]), 1);
+      mbar_init(smem_u32(&sh_bar[warp][1][i]), 1);
     }
     fence_mbar_init();
   }
   balanced_start(
-      p.B, pl.NHG, [&](int b) -> long long { return req_tiles(p, b); }, sh_warp, sh_info);
-
-  Walk walk;
-  walk.g = sh_info[0];
-  walk.g_end = sh_info[1];
-  walk.E = sh_info[2];
-  walk.b = static_cast<int>(sh_info[3]);
-  walk.row0 = sh_info[4] * pl.NHG;
-  walk.T = sh_info[5];
-  walk.hg = 0;
-  walk.S = walk.g < walk.g_end ? req_len(p, walk.b) : 0;
-  walk.L = (walk.S + kTileTokens - 1) / kTileTokens;
-  Seg s;
-
-  if (warp == pl.ncw) {
-    // ------------------------------ producer ------------------------------
-    const uint64_t pol = policy_evict_first();
-    const uint32_t row_bytes = static_cast<uint32_t>(pl.HG * kTile);
-    int slot = 0;
-    uint32_t phase = 0;
-    long long issued = 0;
-    bool ok = true;
-    while (ok && next_seg(walk, p, s)) {
-      const int* table = p.block_table + static_cast<size_t>(s.b) * p.max_blocks;
-      for (int st = s.s0; st < s.s1 && ok; st += pl.slot_tiles) {
-        const int nt = min(pl.slot_tiles, s.s1 - st);
-        size_t off = 0;
-        if (lane < nt) {
-          const int tile = st + lane;
-          const int lb = tile / p.tiles_per_block, sub = tile - lb * p.tiles_per_block;
-          int page = __ldg(table + lb);
-          if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_blocks)) {
-            raise_status(kStatusBadPage);
-            page = 0;
-          }
-          off = ((static_cast<size_t>(page) * p.tiles_per_block + sub) * p.Hkv +
-                 static_cast<size_t>(s.hg) * pl.HG) * kTile;
-        }
-        #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-          if (!__all_sync(kFull, mbar_wait(empty + 8 * slot, phase ^ 1))) {
-            raise_status(kStatusWaitTimeout);
-            ok = false;
-            break;
-          }
-          if (lane == 0) mbar_arrive_expect_tx(full + 8 * slot, row_bytes * nt);
-          __syncwarp();
-          if (lane < nt)
-            bulk_g2s(ring + slot * pl.slot_bytes + lane * row_bytes, (kv ? p.v : p.k) + off,
-                     row_bytes, full + 8 * slot, pol);
-          ++issued;
-          if (++slot == pl.nslots) {
-            slot = 0;
-            phase ^= 1;
-          }
-        }
-      }
-    }
-    // No copy may land after the CTA has exited (see the K1 scan).
-    const long long inflight = min(issued, static_cast<long long>(pl.nslots));
-    for (long long j = 1; j <= inflight; ++j) {
-      const long long idx = issued - j;
-      mbar_wait(full + 8 * static_cast<int>(idx % pl.nslots),
-                static_cast<uint32_t>((idx / pl.nslots) & 1));
-    }
-    return;
+      p.B, pl.NHG, [&](int b) -> long long { return tiles_of(req_len(p, b)); }, sh_warp, sh_info);
+  const long long E = sh_info[2], T = sh_info[5];
+  if (lane < 2) {
+    Walk w;
+    w.g = sh_info[0];
+    w.g_end = sh_info[1];
+    w.b = static_cast<int>(sh_info[3]);
+    w.row0 = sh_info[4] * pl.NHG;
+    w.hg = 0;
+    w.S = w.g < w.g_end ? req_len(p, w.b) : 0;
+    w.L = tiles_of(w.S);
+    sh_walk[warp][lane] = w;
   }
+  __syncwarp();
 
-  // ------------------------------ consumers -------------------------------
-  const int team = warp / pl.TS, ts = warp - team * pl.TS;  // team = (kv head, q-head tile)
-  const int hl = team / pl.NT, j0 = (team - hl * pl.NT) * 8;
-  const int cnt = min(8, pl.G - j0);
-  const int g = lane >> 2, t = lane & 3;
-  float* scratch = reinterpret_cast<float*>(smem + pl.nslots * pl.slot_bytes) +
-                   static_cast<size_t>(team) * (pl.TS / 2) * (kStateBytes / 4);
+  // ---- this warp's copies: unit u in slot u mod units, K and V apart ----
+  const uint32_t ring = smem_u32(smem) + static_cast<uint32_t>(warp * pl.units) * 2 * kUnit;
+  const uint32_t bar_k = smem_u32(&sh_bar[warp][0][0]), bar_v = smem_u32(&sh_bar[warp][1][0]);
+  const uint64_t pol = policy_evict_first();
+  Copier cp;
+  cp.unit = cp.units = 0;
+  const auto copy = [&](const unsigned char* cache, uint32_t tile, int hg, int c, uint32_t dst,
+                        uint32_t bar) {
+    if (lane == 0) mbar_arrive_expect_tx(bar, c * kTile);
+    __syncwarp();
+    if (lane < c)
+      bulk_g2s(dst + lane * kTile,
+               cache + (static_cast<size_t>(tile) * p.Hkv + hg * pl.HG + hl) * kTile, kTile, bar, pol);
+  };
+  int pending = 0;  // units copied and not yet done with
+  for (int i = 0; i < pl.units; ++i) {
+    uint32_t tile;
+    const int c = cp.next(p, &sh_walk[warp][0], ts, tile);
+    if (c == 0) break;
+    copy(p.k, tile, cp.hg, c, ring + i * 2 * kUnit, bar_k + 8 * i);
+    copy(p.v, tile, cp.hg, c, ring + i * 2 * kUnit + kUnit, bar_v + 8 * i);
+    ++pending;
+  }
 
   // Requests without tokens occupy no tiles: CTA (b mod grid) zeroes them.
   for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
@@ -342,163 +386,241 @@ __global__ void __launch_bounds__((kMaxWarps + 1) * 32, 1)
 
   int slot = 0;
   uint32_t phase = 0;
+  // After a wait gave up: waits (each with its limit) for the copies of the
+  // next nk units' K and nv units' V, so that none lands after the CTA's end.
+  const auto drain = [&](int nk, int nv) {
+    for (int k = 0; k < max(nk, nv); ++k) {
+      const bool wrap = slot + k >= pl.units;
+      const int sl = wrap ? slot + k - pl.units : slot + k;
+      const uint32_t ph = wrap ? phase ^ 1u : phase;
+      if (k < nk) mbar_wait(bar_k + 8 * sl, ph);
+      if (k < nv) mbar_wait(bar_v + 8 * sl, ph);
+    }
+    __syncwarp();
+  };
   bool dead = false;  // a wait gave up: empty states from here on (see the K1 scan)
   bool first_seg = true;
-  const auto advance = [&]() {
-    if (++slot == pl.nslots) {
-      slot = 0;
-      phase ^= 1;
-    }
-  };
-
-  while (next_seg(walk, p, s)) {
-    const int hbase = (s.hg * pl.HG + hl) * pl.G + j0;
+  Seg s;
+  long long row_start;
+  while (next_seg(&sh_walk[warp][1], p, s, row_start)) {
+    const long long row_end = row_start + tiles_of(s.S);
+    s.cfirst = range_owner(row_start, T, E);
+    s.nparts = static_cast<int>(range_owner(row_end - 1, T, E) - s.cfirst + 1);
     if (warp == 0 && lane == 0) {
-      if (first_seg && s.nparts > 1 && s.s1 == (s.S + kTileTokens - 1) / kTileTokens)
+      if (first_seg && s.nparts > 1 && row_start + s.s1 == row_end)
         p.ends[blockIdx.x] = make_int2(s.row, s.nparts);
       if (s.s0 == 0) p.row_info[s.row] = make_int2(static_cast<int>(s.cfirst), s.nparts);
     }
     first_seg = false;
-
-    // q fragments (B operand): lane (g, t) holds head g, words 4 i + t.
-    uint32_t qf[8][2];
-    uint32_t qsum_b;        // group sums of q, high and low bf16 parts, as a B operand
-    float start[NG][2];     // -136 Q of heads 2 t, 2 t + 1
-    {
-      const bool has = g < cnt;
-      const __nv_bfloat16* qrow =
-          p.q + (static_cast<size_t>(s.b) * p.Hq + hbase + (has ? g : 0)) * kHeadDim;
-      float qs[4];
-      #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint4 w = has ? __ldg(reinterpret_cast<const uint4*>(qrow + 8 * (4 * i + t)))
-                            : make_uint4(0, 0, 0, 0);
-        // dims (0, 4), (1, 5), (2, 6), (3, 7) of the word
-        qf[2 * i][0] = __byte_perm(w.x, w.z, 0x5410);
-        qf[2 * i][1] = __byte_perm(w.x, w.z, 0x7632);
-        qf[2 * i + 1][0] = __byte_perm(w.y, w.w, 0x5410);
-        qf[2 * i + 1][1] = __byte_perm(w.y, w.w, 0x7632);
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-        float a = 0.f;
-        #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          a += __uint_as_float(u[k] << 16) + __uint_as_float(u[k] & 0xffff0000u);
-        a += __shfl_xor_sync(kFull, a, 1);
-        a += __shfl_xor_sync(kFull, a, 2);
-        qs[i] = a;
-      }
-      float Q[NG];
-      #pragma unroll
-      for (int y = 0; y < NG; ++y) {
-        Q[y] = 0.f;
-        #pragma unroll
-        for (int i = 0; i < 4 / NG; ++i) Q[y] += qs[y * (4 / NG) + i];
-        start[y][0] = -136.f * __shfl_sync(kFull, Q[y], 8 * t);
-        start[y][1] = -136.f * __shfl_sync(kFull, Q[y], 8 * t + 4);
-      }
-      float hi[NG], lo[NG];
-      #pragma unroll
-      for (int y = 0; y < NG; ++y) {
-        hi[y] = __bfloat162float(__float2bfloat16(Q[y]));
-        lo[y] = Q[y] - hi[y];
-      }
-      if constexpr (NG == 4) {
-        const uint32_t h01 = pack_bf16x2(hi[0], hi[1]), h23 = pack_bf16x2(hi[2], hi[3]);
-        const uint32_t l01 = pack_bf16x2(lo[0], lo[1]), l23 = pack_bf16x2(lo[2], lo[3]);
-        qsum_b = t < 2 ? (t == 0 ? h01 : h23) : (t == 2 ? l01 : l23);
-      } else if constexpr (NG == 2) {
-        qsum_b = t == 0 ? pack_bf16x2(hi[0], hi[1]) : (t == 1 ? pack_bf16x2(lo[0], lo[1]) : 0u);
-      } else {
-        qsum_b = t == 0 ? pack_bf16x2(hi[0], lo[0]) : 0u;
-      }
-    }
+    const int hbase = (s.hg * pl.HG + hl) * pl.G + j0;
+    const int units = my_units(s.s1 - s.s0, ts, pl.TS);
+    const int active = min(pl.TS, (s.s1 - s.s0 + 1) / 2);  // warps of the team with a unit
 
     State a;
-    a.m[0] = a.m[1] = -INFINITY;
+    a.m[0] = a.m[1] = kNoRef;
     a.l[0] = a.l[1] = 0.f;
     #pragma unroll
     for (int mt = 0; mt < 8; ++mt) a.acc[mt][0] = a.acc[mt][1] = a.acc[mt][2] = a.acc[mt][3] = 0.f;
-    float cw[4] = {0.f, 0.f, 0.f, 0.f};  // sum_t p_t c_ty: row y = g, heads 2 t, 2 t + 1
 
-    for (int st = s.s0; st < s.s1 && !dead; st += pl.slot_tiles) {
-      const int mine = min(2, min(pl.slot_tiles, s.s1 - st) - 2 * ts);  // tiles of this warp
-      const uint32_t tile0 = static_cast<uint32_t>((2 * ts * pl.HG + hl) * kTile);
-      const uint32_t tile_step = static_cast<uint32_t>(pl.HG * kTile);
-      const int left = s.S - (st + 2 * ts) * kTileTokens;  // valid tokens from tile 0 on
-      float x[2][4];
-
-      if (!__all_sync(kFull, mbar_wait(full + 8 * slot, phase))) {
-        dead = true;
-        break;
+    if (units > 0) {
+      // q fragments (B operand): lane (g, t) holds head g, words 4 i + t, each
+      // as the dim pairs (0, 4), (1, 5), (2, 6), (3, 7) that meet the codes.
+      uint32_t qf[8][2];
+      uint32_t qsum_b;     // 2^-24 Q, high and low bf16 parts, as a B operand
+      float start[NG][2];  // -8 2^-24 Q of heads 2 t, 2 t + 1
+      float fac[2];        // what takes a sum to the score in log2 units
+      {
+        const bool has = g < cnt;
+        const __nv_bfloat16* qrow =
+            p.q + (static_cast<size_t>(s.b) * p.Hq + hbase + (has ? g : 0)) * kHeadDim;
+        uint4 w[4];
+        uint32_t top = 0;  // largest |q| of the head, as bits
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          w[i] = has ? __ldg(reinterpret_cast<const uint4*>(qrow + 8 * (4 * i + t)))
+                     : make_uint4(0, 0, 0, 0);
+          const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+          #pragma unroll
+          for (int k = 0; k < 4; ++k)
+            top = max(top, max(u[k] & 0x7fffu, (u[k] >> 16) & 0x7fffu));
+        }
+        top = max(top, __shfl_xor_sync(kFull, top, 1));
+        top = max(top, __shfl_xor_sync(kFull, top, 2));
+        const int e = max(-100, min(100, static_cast<int>(top >> 7) - 127));
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);  // 2^-e
+        const float up = p.scale_log2 * 16777216.f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        fac[0] = __shfl_sync(kFull, up, 8 * t);
+        fac[1] = __shfl_sync(kFull, up, 8 * t + 4);
+        float Q[NG];
+        #pragma unroll
+        for (int y = 0; y < NG; ++y) Q[y] = 0.f;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+          float q[8];
+          float sum = 0.f;
+          #pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            q[2 * k] = __uint_as_float(u[k] << 16) * down;
+            q[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u) * down;
+          }
+          #pragma unroll
+          for (int k = 0; k < 8; ++k) sum += q[k];
+          qf[2 * i][0] = pack_half2(q[0], q[4]);
+          qf[2 * i][1] = pack_half2(q[1] * 0.0625f, q[5] * 0.0625f);
+          qf[2 * i + 1][0] = pack_half2(q[2], q[6]);
+          qf[2 * i + 1][1] = pack_half2(q[3] * 0.0625f, q[7] * 0.0625f);
+          sum += __shfl_xor_sync(kFull, sum, 1);
+          sum += __shfl_xor_sync(kFull, sum, 2);
+          Q[i * NG / 4] += sum;
+        }
+        float hi[NG], lo[NG];
+        #pragma unroll
+        for (int y = 0; y < NG; ++y) {
+          Q[y] *= 1.f / 16777216.f;
+          start[y][0] = -8.f * __shfl_sync(kFull, Q[y], 8 * t);
+          start[y][1] = -8.f * __shfl_sync(kFull, Q[y], 8 * t + 4);
+          hi[y] = __bfloat162float(__float2bfloat16(Q[y]));
+          lo[y] = Q[y] - hi[y];
+        }
+        if constexpr (NG == 4) {
+          const uint32_t h01 = pack_bf16x2(hi[0], hi[1]), h23 = pack_bf16x2(hi[2], hi[3]);
+          const uint32_t l01 = pack_bf16x2(lo[0], lo[1]), l23 = pack_bf16x2(lo[2], lo[3]);
+          qsum_b = t < 2 ? (t == 0 ? h01 : h23) : (t == 2 ? l01 : l23);
+        } else if constexpr (NG == 2) {
+          qsum_b = t == 0 ? pack_bf16x2(hi[0], hi[1]) : (t == 1 ? pack_bf16x2(lo[0], lo[1]) : 0u);
+        } else {
+          qsum_b = t == 0 ? pack_bf16x2(hi[0], lo[0]) : 0u;
+        }
       }
-      if (mine > 0) {
-        const uint32_t kb = ring + slot * pl.slot_bytes + tile0;
+      float cw[4] = {0.f, 0.f, 0.f, 0.f};  // sum_t p_t c_ty: row y = g, heads 2 t, 2 t + 1
+
+      for (int i = 0; i < units && !dead; ++i) {
+        const int tile_no = s.s0 + 2 * (i * pl.TS + ts);
+        const int left = s.S - tile_no * kTileTokens;  // valid tokens from here on
+        const bool two = tile_no + 1 < s.s1;
+        const uint32_t kb = ring + static_cast<uint32_t>(slot) * 2 * kUnit, vb = kb + kUnit;
+        float x[2][4];
+
+        // ---- scores of two tiles ----
+        if (!__all_sync(kFull, mbar_wait(bar_k + 8 * slot, phase))) {
+          drain(pending, pending);
+          dead = true;
+          break;
+        }
         #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          x[j][0] = x[j][1] = x[j][2] = x[j][3] = -INFINITY;
-          if (j < mine) {
-            const uint32_t tb = kb + j * tile_step;
-            const uint4 wa = lds128(tb + 64 * g + 16 * t), wb = lds128(tb + 512 + 64 * g + 16 * t);
-            const uint32_t ua[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
-            float sa[NG], sb[NG];
-            load_scales<NG>(tb + scale_at(0, 0, NG) + 2 * NG * g, sa);
-            load_scales<NG>(tb + scale_at(8, 0, NG) + 2 * NG * g, sb);
-            uint32_t ca, cb;
-            if constexpr (NG == 4) {
-              ca = lds32(tb + k_centre_at(0, 0, NG) + 8 * g + 4 * (t & 1));
-              cb = lds32(tb + k_centre_at(8, 0, NG) + 8 * g + 4 * (t & 1));
-            } else if constexpr (NG == 2) {
-              ca = lds32(tb + k_centre_at(0, 0, NG) + 4 * g);
-              cb = lds32(tb + k_centre_at(8, 0, NG) + 4 * g);
-            } else {
-              ca = lds16(tb + k_centre_at(0, 0, NG) + 2 * g) * 0x10001u;
-              cb = lds16(tb + k_centre_at(8, 0, NG) + 2 * g) * 0x10001u;
-            }
-            float sc[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_bf16_16816(sc, ca, cb, 0u, 0u, qsum_b, 0u);
+          // (a unit without a second tile reads what the slot held before; its
+          // scores are masked like those behind the last token)
+          const uint32_t tb = kb + j * kTile;
+          const uint4 wa = lds128(tb + 64 * g + 16 * t), wb = lds128(tb + 512 + 64 * g + 16 * t);
+          const uint32_t ua[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
+          float sa[NG], sb[NG];
+          load_scales<NG>(tb + scale_at(0, 0, NG) + 2 * NG * g, sa);
+          load_scales<NG>(tb + scale_at(8, 0, NG) + 2 * NG * g, sb);
+          uint32_t ca, cb;
+          if constexpr (NG == 4) {
+            ca = lds32(tb + k_centre_at(0, 0, NG) + 8 * g + 4 * (t & 1));
+            cb = lds32(tb + k_centre_at(8, 0, NG) + 8 * g + 4 * (t & 1));
+          } else if constexpr (NG == 2) {
+            ca = lds32(tb + k_centre_at(0, 0, NG) + 4 * g);
+            cb = lds32(tb + k_centre_at(8, 0, NG) + 4 * g);
+          } else {
+            ca = lds16(tb + k_centre_at(0, 0, NG) + 2 * g) * 0x10001u;
+            cb = lds16(tb + k_centre_at(8, 0, NG) + 2 * g) * 0x10001u;
+          }
+          float sc[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_bf16_16816(sc, ca, cb, 0u, 0u, qsum_b, 0u);
+          #pragma unroll
+          for (int y = 0; y < NG; ++y) {
+            float d[4] = {start[y][0], start[y][1], start[y][0], start[y][1]};
             #pragma unroll
-            for (int y = 0; y < NG; ++y) {
-              float d[4] = {start[y][0], start[y][1], start[y][0], start[y][1]};
-              #pragma unroll
-              for (int i = y * (4 / NG); i < (y + 1) * (4 / NG); ++i) {
-                mma_bf16_16816(d, code_pair(ua[i], 0), code_pair(ub[i], 0), code_pair(ua[i], 1),
-                               code_pair(ub[i], 1), qf[2 * i][0], qf[2 * i][1]);
-                mma_bf16_16816(d, code_pair(ua[i], 2), code_pair(ub[i], 2), code_pair(ua[i], 3),
-                               code_pair(ub[i], 3), qf[2 * i + 1][0], qf[2 * i + 1][1]);
-              }
-              sc[0] += sa[y] * d[0];
-              sc[1] += sa[y] * d[1];
-              sc[2] += sb[y] * d[2];
-              sc[3] += sb[y] * d[3];
+            for (int k = y * (4 / NG); k < (y + 1) * (4 / NG); ++k) {
+              mma_f16_16816(d, low_codes(ua[k]), low_codes(ub[k]), high_codes(ua[k]),
+                            high_codes(ub[k]), qf[2 * k][0], qf[2 * k][1]);
+              mma_f16_16816(d, low_codes(ua[k] >> 8), low_codes(ub[k] >> 8), high_codes(ua[k] >> 8),
+                            high_codes(ub[k] >> 8), qf[2 * k + 1][0], qf[2 * k + 1][1]);
             }
-            const int nv = left - j * kTileTokens;
-            x[j][0] = g < nv ? sc[0] * p.scale_log2 : -INFINITY;
-            x[j][1] = g < nv ? sc[1] * p.scale_log2 : -INFINITY;
-            x[j][2] = g + 8 < nv ? sc[2] * p.scale_log2 : -INFINITY;
-            x[j][3] = g + 8 < nv ? sc[3] * p.scale_log2 : -INFINITY;
+            sc[0] += sa[y] * d[0];
+            sc[1] += sa[y] * d[1];
+            sc[2] += sb[y] * d[2];
+            sc[3] += sb[y] * d[3];
+          }
+          #pragma unroll
+          for (int k = 0; k < 4; ++k) x[j][k] = sc[k] * fac[k & 1];
+        }
+        if (left < 2 * kTileTokens || !two) {
+          const int nv = two ? left : min(left, kTileTokens);
+          #pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            if (j * kTileTokens + g >= nv) x[j][0] = x[j][1] = -INFINITY;
+            if (j * kTileTokens + g + 8 >= nv) x[j][2] = x[j][3] = -INFINITY;
           }
         }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(empty + 8 * slot);
-      advance();
+        __syncwarp();  // every lane has read the K slot: refill it
+        uint32_t next_tile;
+        const int next_c = cp.next(p, &sh_walk[warp][0], ts, next_tile);
+        if (next_c) copy(p.k, next_tile, cp.hg, next_c, kb, bar_k + 8 * slot);
 
-      if (mine > 0) {
-        float mx[2];
-        #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          mx[n] = fmaxf(fmaxf(x[0][n], x[0][2 + n]), fmaxf(x[1][n], x[1][2 + n]));
-          #pragma unroll
-          for (int off = 4; off < 32; off <<= 1)
-            mx[n] = fmaxf(mx[n], __shfl_xor_sync(kFull, mx[n], off));
+        // ---- weights, and the sum over V ----
+        if (!__all_sync(kFull, mbar_wait(bar_v + 8 * slot, phase))) {
+          drain(pending + (next_c ? 1 : 0), pending);
+          dead = true;
+          break;
         }
-        // The running maximum moves only when a score passes it by more than
-        // kThreshold: weights stay below 2^8 and most tiles rescale nothing.
-        if (__any_sync(kFull, mx[0] > a.m[0] + kThreshold || mx[1] > a.m[1] + kThreshold)) {
+        uint32_t pw[2][2], bw[2][2][NG];  // weights (bf16), and times the scales (fp16)
+        #pragma unroll 1
+        for (int pass = 0;; ++pass) {
+          float sm = 0.f;
+          uint32_t over = 0u;  // largest fp16 weight
+          float l[2] = {0.f, 0.f}, w[2][4];
+          #pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float sa[NG], sb[NG];
+            load_scales<NG>(vb + j * kTile + scale_at(0, 0, NG) + 2 * NG * g, sa);
+            load_scales<NG>(vb + j * kTile + scale_at(8, 0, NG) + 2 * NG * g, sb);
+            if (left < 2 * kTileTokens || !two) {
+              // what lies behind the last token may be anything
+              const int nv = two ? left : min(left, kTileTokens);
+              #pragma unroll
+              for (int y = 0; y < NG; ++y) {
+                if (j * kTileTokens + g >= nv) sa[y] = 0.f;
+                if (j * kTileTokens + g + 8 >= nv) sb[y] = 0.f;
+              }
+            }
+            #pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              w[j][k] = exp2_approx(x[j][k] - a.m[k & 1]);
+              l[k & 1] += w[j][k];
+            }
+            pw[j][0] = pack_bf16x2(w[j][0], w[j][1]);
+            pw[j][1] = pack_bf16x2(w[j][2], w[j][3]);
+            #pragma unroll
+            for (int y = 0; y < NG; ++y) {
+              sm = fmaxf(sm, fmaxf(sa[y], sb[y]));
+              bw[j][0][y] = pack_half2(w[j][0] * sa[y], w[j][1] * sa[y]);
+              bw[j][1][y] = pack_half2(w[j][2] * sb[y], w[j][3] * sb[y]);
+              over = max_half2(over, max_half2(bw[j][0][y], bw[j][1][y]));
+            }
+          }
+          // 2^15 in either half, or a weight sum that nears fp32's range
+          const bool big = (over & 0xffffu) >= 0x7800u || over >= 0x78000000u ||
+                           l[0] > 1e30f || l[1] > 1e30f;
+          if (pass == 1 || !__any_sync(kFull, big)) {
+            a.l[0] += l[0];
+            a.l[1] += l[1];
+            break;
+          }
+          #pragma unroll
+          for (int off = 4; off < 32; off <<= 1) sm = fmaxf(sm, __shfl_xor_sync(kFull, sm, off));
+          const float room = __log2f(fminf(fmaxf(sm, 1e-18f), 1e30f)) - 9.f;
           #pragma unroll
           for (int n = 0; n < 2; ++n) {
-            const float m = fmaxf(a.m[n], mx[n]);
-            const float f = a.m[n] == -INFINITY ? 0.f : exp2_approx(a.m[n] - m);
+            float mx = fmaxf(fmaxf(x[0][n], x[0][2 + n]), fmaxf(x[1][n], x[1][2 + n]));
+            #pragma unroll
+            for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, off));
+            const float m = fmaxf(a.m[n], mx + room);
+            const float f = exp2_approx(a.m[n] - m);
             a.m[n] = m;
             a.l[n] *= f;
             cw[n] *= f;
@@ -510,82 +632,45 @@ __global__ void __launch_bounds__((kMaxWarps + 1) * 32, 1)
           }
         }
         #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            x[j][i] = exp2_approx(x[j][i] - a.m[i & 1]);
-            a.l[i & 1] += x[j][i];
-          }
-      }
-
-      if (!__all_sync(kFull, mbar_wait(full + 8 * slot, phase))) {
-        dead = true;
-        break;
-      }
-      if (mine > 0) {
-        const uint32_t vb = ring + slot * pl.slot_bytes + tile0;
-        #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          if (j < mine) {
-            const uint32_t tb = vb + j * tile_step;
-            const uint32_t va = tb + 128 * t + 16 * (g ^ (2 * t));
-            const uint4 wa = lds128(va), wb = lds128(va + 512);
-            const uint32_t ua[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
-            float sa[NG], sb[NG];
-            load_scales<NG>(tb + scale_at(0, 0, NG) + 2 * NG * g, sa);
-            load_scales<NG>(tb + scale_at(8, 0, NG) + 2 * NG * g, sb);
-            uint32_t ca = 0u, cb = 0u;
-            if (g < NG) {
-              ca = lds32(tb + v_centre_at(0, 0, NG) + 32 * g + 4 * t);
-              cb = lds32(tb + v_centre_at(8, 0, NG) + 32 * g + 4 * t);
-            }
-            const int nv = left - j * kTileTokens;
-            if (nv < kTileTokens) {
-              // what lies behind the last token may be anything: no scale, no centre
-              #pragma unroll
-              for (int y = 0; y < NG; ++y) {
-                if (g >= nv) sa[y] = 0.f;
-                if (g + 8 >= nv) sb[y] = 0.f;
-              }
-              if (2 * t >= nv) ca = 0u; else if (2 * t + 1 >= nv) ca &= 0xffffu;
-              if (2 * t + 8 >= nv) cb = 0u; else if (2 * t + 9 >= nv) cb &= 0xffffu;
-            }
-            mma_bf16_16816(cw, ca, 0u, cb, 0u, movmatrix_trans(pack_bf16x2(x[j][0], x[j][1])),
-                           movmatrix_trans(pack_bf16x2(x[j][2], x[j][3])));
+          if (j == 1 && !two) break;
+          const uint32_t tb = vb + j * kTile;
+          const uint32_t va = tb + 128 * t + 16 * (g ^ (2 * t));
+          const uint4 wa = lds128(va), wb = lds128(va + 512);
+          const uint32_t ua[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
+          uint32_t ca = 0u, cb = 0u;
+          if (g < NG) {
+            ca = lds32(tb + v_centre_at(0, 0, NG) + 32 * g + 4 * t);
+            cb = lds32(tb + v_centre_at(8, 0, NG) + 32 * g + 4 * t);
+          }
+          const int nv = left - j * kTileTokens;
+          if (nv < kTileTokens) {
+            if (2 * t >= nv) ca = 0u; else if (2 * t + 1 >= nv) ca &= 0xffffu;
+            if (2 * t + 8 >= nv) cb = 0u; else if (2 * t + 9 >= nv) cb &= 0xffffu;
+          }
+          mma_bf16_16816(cw, ca, 0u, cb, 0u, movmatrix_trans(pw[j][0]), movmatrix_trans(pw[j][1]));
+          #pragma unroll
+          for (int y = 0; y < NG; ++y) {
+            const uint32_t b0 = movmatrix_trans(bw[j][0][y]), b1 = movmatrix_trans(bw[j][1][y]);
             #pragma unroll
-            for (int y = 0; y < NG; ++y) {
-              const uint32_t b0 = movmatrix_trans(pack_bf16x2(x[j][0] * sa[y], x[j][1] * sa[y]));
-              const uint32_t b1 = movmatrix_trans(pack_bf16x2(x[j][2] * sb[y], x[j][3] * sb[y]));
-              #pragma unroll
-              for (int i = y * (4 / NG); i < (y + 1) * (4 / NG); ++i)
-                #pragma unroll
-                for (int u = 0; u < 2; ++u)
-                  mma_bf16_16816(a.acc[2 * i + u], centred(code_pair(ua[i], 2 * u)),
-                                 centred(code_pair(ua[i], 2 * u + 1)),
-                                 centred(code_pair(ub[i], 2 * u)),
-                                 centred(code_pair(ub[i], 2 * u + 1)), b0, b1);
+            for (int k = y * (4 / NG); k < (y + 1) * (4 / NG); ++k) {
+              mma_f16_16816(a.acc[2 * k], low_centred(ua[k]), high_centred(ua[k]),
+                            low_centred(ub[k]), high_centred(ub[k]), b0, b1);
+              mma_f16_16816(a.acc[2 * k + 1], low_centred(ua[k] >> 8), high_centred(ua[k] >> 8),
+                            low_centred(ub[k] >> 8), high_centred(ub[k] >> 8), b0, b1);
             }
           }
         }
+        __syncwarp();  // every lane has read the V slot
+        if (next_c) copy(p.v, next_tile, cp.hg, next_c, vb, bar_v + 8 * slot);
+        else --pending;
+        if (++slot == pl.units) {
+          slot = 0;
+          phase ^= 1;
+        }
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(empty + 8 * slot);
-      advance();
-    }
 
-    // ---- segment epilogue ----
-    if (dead) {
-      if (lane == 0) raise_status(kStatusWaitTimeout);
-      a.m[0] = a.m[1] = -INFINITY;
-      a.l[0] = a.l[1] = 0.f;
-      cw[0] = cw[1] = 0.f;
-      #pragma unroll
-      for (int mt = 0; mt < 8; ++mt)
-        a.acc[mt][0] = a.acc[mt][1] = a.acc[mt][2] = a.acc[mt][3] = 0.f;
-    }
-    // Teams whose segment fits in one warp's tiles skip the meeting.
-    const int active = min(pl.TS, (min(pl.slot_tiles, s.s1 - s.s0) + 1) / 2);
-    if (ts < active) {
+      // ---- the warp's own sums ----
       #pragma unroll
       for (int n = 0; n < 2; ++n) {
         #pragma unroll
@@ -594,24 +679,68 @@ __global__ void __launch_bounds__((kMaxWarps + 1) * 32, 1)
         for (int y = 0; y < NG; ++y) {
           const float c = __shfl_sync(kFull, cw[n], 4 * y + t);
           #pragma unroll
-          for (int i = y * (4 / NG); i < (y + 1) * (4 / NG); ++i)
+          for (int k = y * (4 / NG); k < (y + 1) * (4 / NG); ++k)
             #pragma unroll
             for (int u = 0; u < 2; ++u) {
-              a.acc[2 * i + u][n] += c;
-              a.acc[2 * i + u][2 + n] += c;
+              a.acc[2 * k + u][n] += c;
+              a.acc[2 * k + u][2 + n] += c;
             }
         }
       }
     }
+    if (dead) {
+      if (lane == 0) raise_status(kStatusWaitTimeout);
+      a.m[0] = a.m[1] = -INFINITY;
+      a.l[0] = a.l[1] = 0.f;
+      #pragma unroll
+      for (int mt = 0; mt < 8; ++mt)
+        a.acc[mt][0] = a.acc[mt][1] = a.acc[mt][2] = a.acc[mt][3] = 0.f;
+    }
+
+    // ---- the team meets: halves hand over to halves, a few words at a time ----
     if (active > 1) {
       for (int off = pl.TS / 2; off >= 1; off >>= 1) {
         if (off >= active) continue;  // uniform over the team
-        if (ts >= off && ts < 2 * off && ts < active)
-          put_state(a, scratch + (ts - off) * (kStateBytes / 4), lane);
-        group_barrier(1 + team, 32 * pl.TS);
-        if (ts < off && ts + off < active)
-          merge_state(a, scratch + ts * (kStateBytes / 4), lane);
-        group_barrier(1 + team, 32 * pl.TS);
+        const bool gives = ts >= off && ts < 2 * off && ts < active;
+        const bool takes = ts < off && ts + off < active;
+        float* box = scratch + (gives ? ts - off : (takes ? ts : 0)) * kPassWords * 32 + lane;
+        float fa[2], fo[2];
+        #pragma unroll
+        for (int pass = 0; pass < 5; ++pass) {
+          if (gives) {
+            if (pass == 0) {
+              #pragma unroll
+              for (int n = 0; n < 2; ++n) {
+                box[n * 32] = a.m[n];
+                box[(2 + n) * 32] = a.l[n];
+              }
+            } else {
+              #pragma unroll
+              for (int k = 0; k < kPassWords; ++k)
+                box[k * 32] = a.acc[2 * (pass - 1) + k / 4][k % 4];
+            }
+          }
+          group_barrier(1 + team, 32 * pl.TS);
+          if (takes) {
+            if (pass == 0) {
+              #pragma unroll
+              for (int n = 0; n < 2; ++n) {
+                const float mo = box[n * 32], m = fmaxf(a.m[n], mo);
+                fa[n] = a.m[n] == -INFINITY ? 0.f : exp2_approx(a.m[n] - m);
+                fo[n] = mo == -INFINITY ? 0.f : exp2_approx(mo - m);
+                a.m[n] = m;
+                a.l[n] = a.l[n] * fa[n] + box[(2 + n) * 32] * fo[n];
+              }
+            } else {
+              #pragma unroll
+              for (int k = 0; k < kPassWords; ++k) {
+                float& v = a.acc[2 * (pass - 1) + k / 4][k % 4];
+                v = v * fa[k & 1] + box[k * 32] * fo[k & 1];
+              }
+            }
+          }
+          group_barrier(1 + team, 32 * pl.TS);
+        }
       }
     }
     if (ts != 0) continue;
@@ -628,7 +757,9 @@ __global__ void __launch_bounds__((kMaxWarps + 1) * 32, 1)
               make_uint2(pack_bf16x2(a.acc[2 * y][n] * inv, a.acc[2 * y][2 + n] * inv),
                          pack_bf16x2(a.acc[2 * y + 1][n] * inv, a.acc[2 * y + 1][2 + n] * inv));
       } else {
-        const size_t idx = static_cast<size_t>(s.slot) * (pl.HG * pl.G) + hl * pl.G + j0 + head;
+        // slot of the partial state: this CTA's, of the row's (K1's layout)
+        const size_t idx = (static_cast<size_t>(blockIdx.x) + s.row) * (pl.HG * pl.G) + hl * pl.G +
+                           j0 + head;
         if (g == 0) {
           p.part_m[idx] = a.m[n];
           p.part_l[idx] = a.l[n];
@@ -722,20 +853,20 @@ int make_plan(int Hq, int Hkv, int group, Plan* p) {
   p->G = Hq / Hkv;
   p->NT = (p->G + 7) / 8;
   if (p->NT > kMaxWarps) return -1;
-  // kv heads per row: up to 8 warps' worth, so that two warps can share each
-  // head's tokens; then as many warps per head as 16 allow.
+  // kv heads per row: up to 8 warps' worth, so that at least two warps share a
+  // head's tokens (with up to 64 q heads per kv head); then as many warps per
+  // head as 16 allow.
   p->HG = 1;
   for (int d = 1; d <= Hkv && d * p->NT <= 8; ++d)
     if (Hkv % d == 0) p->HG = d;
   p->NHG = Hkv / p->HG;
   p->TS = 1;
   while (2 * p->TS * p->HG * p->NT <= kMaxWarps) p->TS *= 2;
-  p->ncw = p->HG * p->NT * p->TS;
-  p->slot_tiles = 2 * p->TS;
-  p->slot_bytes = p->slot_tiles * p->HG * tile_bytes(group);
-  const int scratch = p->HG * p->NT * (p->TS / 2) * kStateBytes;
-  p->nslots = std::min(kMaxSlots, (kSmemLimit - 2048 - scratch) / p->slot_bytes);
-  p->smem = p->nslots * p->slot_bytes + scratch;
+  p->warps = p->HG * p->NT * p->TS;
+  const int unit_bytes = 4 * tile_bytes(group);  // K and V of two tiles
+  const int scratch = p->HG * p->NT * (p->TS / 2) * kPassWords * 32 * 4;
+  p->units = std::min(kMaxUnits, (kSmemLimit - kSmemStatic - scratch) / (p->warps * unit_bytes));
+  p->smem = p->warps * p->units * unit_bytes + scratch;
   return 0;
 }
 
@@ -759,7 +890,7 @@ DeviceOnce g_smem_once;
 
 cudaError_t set_smem_limits() {
   return g_smem_once.run([] {
-    const int bytes = kSmemLimit - 2048;
+    const int bytes = kSmemLimit - kSmemStatic;
     cudaError_t e = cudaFuncSetAttribute(kv4_decode_kernel<1>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e == cudaSuccess)
@@ -836,7 +967,7 @@ cudaError_t kv4_decode_launch(const gqa_bf16* q, const unsigned char* k_cache,
   p.num_blocks = num_blocks;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.pl = pl;
-  const int threads = (pl.ncw + 1) * 32;
+  const int threads = pl.warps * 32;
   if (group == 32) kv4_decode_kernel<4><<<grid, threads, pl.smem, stream>>>(p);
   else if (group == 64) kv4_decode_kernel<2><<<grid, threads, pl.smem, stream>>>(p);
   else kv4_decode_kernel<1><<<grid, threads, pl.smem, stream>>>(p);
