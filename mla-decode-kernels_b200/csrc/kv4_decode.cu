@@ -10,26 +10,33 @@
 // scales are folded into the softmax weights of each group, and both centre
 // terms are one small tensor-core product per tile.
 //   * K: a masked nibble is the fp16 subnormal n 2^-24 or 16 n 2^-24 as it
-//     stands.  q enters in fp16, divided by a power of two per head so that
-//     its largest element is in [1, 2) (and by 16 more where it meets 16 n);
-//     the accumulator starts at -8 Q_y.  A q element below 2^-17 of its
-//     head's largest loses bits there, 2^-25 of that largest at most.
-//   * V: the nibble becomes 1024 + n or 1024 + 16 n in fp16 by one and-or,
-//     then n - 8 by one packed operation, exactly.  (Codes left positive
-//     would pile up a sum that the centre term takes away again: over a long
-//     context fp32 loses the difference.)  The weights p_t s_ty are rounded
-//     to fp16, 2^-11 instead of bf16's 2^-8.
+//     stands, and a whole byte (16 n' + n) 2^-24.  q enters in fp16, divided
+//     by a power of two per head so that its largest element is in [1, 2)
+//     (and by 16 more where it meets 16 n); where n' comes with n in one byte,
+//     n meets q - q' / 16 instead, which is the only one of four that fp16
+//     rounds (2^-12).  A q element below 2^-17 of its head's largest loses
+//     bits, 2^-25 of that largest at most.  The offset 8 is taken off by the
+//     centres' product, as the centre -8 s.
+//   * V: the same three patterns less 8, 128 and 136 (one packed subtraction,
+//     exact), so that the sums stay small: left positive they would pile up
+//     what the centres take away again, and over a long context fp32 loses
+//     the difference.  The byte's sum is 16 out' + out; the head's end
+//     resolves it.  The weights p_t s_ty are rounded to fp16, 2^-11.
 // The softmax reference M of a head is no running maximum but any value that
 // keeps the fp16 weights in range: it is set so that the largest p s is 2^9
 // and moves only when one passes 2^15, so the common step takes no maximum
 // and rescales nothing.
 //
 // Layout (one persistent CTA per SM, the balanced schedule of
-// gqa_balance.cuh, cut rows merged by the cut-row merge kernel): HG x NT x TS
-// = up to 16 warps: kv head, 8 of its q heads, and every TS-th pair of tiles.
-// Each warp copies its own tiles (cp.async.bulk, one per tile) into its own
-// ring and refills a slot as soon as it has read it, so no warp waits for
-// another until the TS warps of a head meet at the end of a segment.
+// gqa_balance.cuh, cut rows merged by the cut-row merge kernel):
+//   * up to 16 consumer warps, HG x NT x TS: kv head, 8 of its q heads, and
+//     every TS-th pair of tiles; the TS warps of a head keep their own state
+//     and meet at the end of a segment;
+//   * one copy warp: a row of HG kv heads is contiguous in the cache, so one
+//     cp.async.bulk brings a tile of all of them.  A ring slot holds K or V
+//     of 2 TS tiles.  The consumers need more registers than 17 warps can
+//     share evenly, so the copy warp's group gives up most of its own.
+#include <cuda_fp16.h>
 #include <math.h>
 
 #include <algorithm>
@@ -53,7 +60,11 @@ namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kMaxWarps = 16;
-constexpr int kMaxUnits = 4;                 // units (pairs of tiles) in a warp's ring
+constexpr int kMaxSlots = 16;
+constexpr int kThreads = (kMaxWarps + 4) * 32;  // and the copy warp's group
+// Registers: 640 threads at 96 are launched; 512 consumer threads at 112 and
+// 128 at 24 are 60416 of those 61440.
+constexpr int kConsumerRegs = 112, kCopyRegs = 24;
 constexpr int kSmemLimit = 227 * 1024;
 constexpr int kSmemStatic = 3 * 1024;        // bound of the kernel's static shared memory
 constexpr int kPassWords = 8;                // floats per lane handed over at once at a meeting
@@ -64,8 +75,7 @@ __device__ __forceinline__ void raise_status(int bits) { atomicOr(&g_kv4_status,
 // How a launch maps to warps and shared memory (no device state).
 struct Plan {
   int G, NT, HG, NHG, TS, warps;
-  int units;  // ring depth
-  int smem;
+  int slot_tiles, slot_bytes, nslots, smem;
 };
 
 struct DecodeParams {
@@ -109,23 +119,17 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-// K: codes j and j + 4 (j even), or 16 times codes j + 1 and j + 5, of a word
-// shifted by 4 j, in units of 2^-24.
-__device__ __forceinline__ uint32_t low_codes(uint32_t w) { return w & 0x000f000fu; }
-__device__ __forceinline__ uint32_t high_codes(uint32_t w) { return w & 0x00f000f0u; }
+// Codes as fp16 in units of 2^-24.  Of a 32-bit word of eight codes: n of
+// nibbles 0 and 4; 16 n of nibbles 1 and 5; bytes 1 and 3 (16 n' + n: nibbles
+// 3 and 7, 2 and 6); and of those, n.
+__device__ __forceinline__ uint32_t codes_n(uint32_t w) { return w & 0x000f000fu; }
+__device__ __forceinline__ uint32_t codes_16n(uint32_t w) { return w & 0x00f000f0u; }
+__device__ __forceinline__ uint32_t codes_byte(uint32_t w) { return __byte_perm(w, 0u, 0x4341); }
 
-// V: the same codes as n - 8 in fp16.  1024 + n and 1024 + 16 n are exact
-// (fp16 counts in ones from 1024 on), and so is what follows.
-__device__ __forceinline__ uint32_t low_centred(uint32_t w) {
+// a - b in fp16 (exact here: multiples of 2^-24 below 2^-16).
+__device__ __forceinline__ uint32_t sub_half2(uint32_t a, uint32_t b) {
   uint32_t r;
-  asm("lop3.b32 %0, %1, 0x000f000f, 0x64006400, 0xea;" : "=r"(r) : "r"(w));
-  asm("sub.rn.f16x2 %0, %0, %1;" : "+r"(r) : "r"(0x64086408u));  // - 1032
-  return r;
-}
-__device__ __forceinline__ uint32_t high_centred(uint32_t w) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, 0x00f000f0, 0x64006400, 0xea;" : "=r"(r) : "r"(w));
-  asm("fma.rn.f16x2 %0, %0, %1, %2;" : "+r"(r) : "r"(0x2c002c00u), "r"(0xd480d480u));  // / 16 - 72
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 
@@ -151,33 +155,56 @@ __device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// The NG bf16 scales of one token as floats.
+// The NG bf16 scales (or centres) of one token, as stored: words of two.
 template <int NG>
-__device__ __forceinline__ void load_scales(uint32_t a, float (&s)[NG]) {
+struct Scales {
+  uint32_t w[(NG + 1) / 2];
+  __device__ __forceinline__ void load(uint32_t a) {
+    if constexpr (NG == 4)
+      asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a));
+    else if constexpr (NG == 2)
+      w[0] = lds32(a);
+    else
+      w[0] = lds16(a) * 0x10001u;
+  }
+  __device__ __forceinline__ float operator[](int y) const {
+    return __uint_as_float(y & 1 ? w[y / 2] & 0xffff0000u : w[y / 2] << 16);
+  }
+  // What lane t holds of them as an A operand whose columns are (high, low)
+  // copies: 0 .. NG - 1, 0 .. NG - 1.
+  __device__ __forceinline__ uint32_t operand(int t) const {
+    if constexpr (NG == 4) return t & 1 ? w[1] : w[0];
+    return w[0];
+  }
+};
+
+// Values Q_y as the B operand that meets Scales::operand: their high bf16
+// parts, then what those leave.
+template <int NG>
+__device__ __forceinline__ uint32_t high_low(const float (&Q)[NG], int t) {
+  float hi[NG], lo[NG];
+  #pragma unroll
+  for (int y = 0; y < NG; ++y) {
+    hi[y] = __bfloat162float(__float2bfloat16(Q[y]));
+    lo[y] = Q[y] - hi[y];
+  }
   if constexpr (NG == 4) {
-    uint32_t x, y;
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(x), "=r"(y) : "r"(a));
-    s[0] = __uint_as_float(x << 16);
-    s[1] = __uint_as_float(x & 0xffff0000u);
-    s[2] = __uint_as_float(y << 16);
-    s[3] = __uint_as_float(y & 0xffff0000u);
+    const uint32_t h01 = pack_bf16x2(hi[0], hi[1]), h23 = pack_bf16x2(hi[2], hi[3]);
+    const uint32_t l01 = pack_bf16x2(lo[0], lo[1]), l23 = pack_bf16x2(lo[2], lo[3]);
+    return t < 2 ? (t == 0 ? h01 : h23) : (t == 2 ? l01 : l23);
   } else if constexpr (NG == 2) {
-    const uint32_t x = lds32(a);
-    s[0] = __uint_as_float(x << 16);
-    s[1] = __uint_as_float(x & 0xffff0000u);
+    return t == 0 ? pack_bf16x2(hi[0], hi[1]) : (t == 1 ? pack_bf16x2(lo[0], lo[1]) : 0u);
   } else {
-    s[0] = __uint_as_float(lds16(a) << 16);
+    return t == 0 ? pack_bf16x2(hi[0], lo[0]) : 0u;
   }
 }
 
 struct Seg {
-  int b, hg, row, S, s0, s1, nparts;
-  long long cfirst;
+  int b, hg, row, S, s0, s1;
 };
 
 // The CTA's share of the balanced schedule, as segments (one row, a range of
-// its tiles).  Every warp keeps two in shared memory, one ahead of the other:
-// for the copies and for the tiles it works on.
+// its tiles).  Every warp keeps its own, in shared memory.
 struct Walk {
   long long g, g_end, row0;
   int b, hg, S, L;
@@ -236,64 +263,6 @@ __device__ __forceinline__ void group_barrier(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
 
-// Units (pairs of tiles) of a segment of n tiles that warp ts of TS takes:
-// units ts, ts + TS, ...
-__device__ __forceinline__ int my_units(int n, int ts, int TS) {
-  const int units = (n + 1) / 2;
-  return ts < units ? (units - ts + TS - 1) / TS : 0;
-}
-
-// The copies of one warp: the physical tiles of its units, in order, across
-// segments.  Lane i holds the tile of unit first + i / 2, i % 2 of its pair;
-// the next 16 units' block ids are loaded while these are used.
-struct Copier {
-  const int* table;  // the segment's row of the block table
-  int n, s0, hg;     // tiles of the segment, its first tile, its kv-head group
-  int unit, units;   // next unit of this warp, and how many there are
-  uint32_t cur, nxt; // physical tiles (block * tiles per block + place in it)
-
-  __device__ __forceinline__ uint32_t look_up(const DecodeParams& p, int first, int ts) const {
-    const int lane = threadIdx.x & 31;
-    const int u = first + lane / 2;
-    const int tile = 2 * (u * p.pl.TS + ts) + (lane & 1);
-    if (u >= units || tile >= n) return 0;
-    const int lb = (s0 + tile) / p.tiles_per_block, sub = s0 + tile - lb * p.tiles_per_block;
-    int page = ld_nc_s32(table + lb);
-    if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_blocks)) {
-      raise_status(kStatusBadPage);
-      page = 0;
-    }
-    return static_cast<uint32_t>(page) * static_cast<uint32_t>(p.tiles_per_block) + sub;
-  }
-
-  // Tiles of the next unit (1 or 2; 0: no more), each lane's parity's tile in
-  // `tile`.
-  __device__ __forceinline__ int next(const DecodeParams& p, Walk* walk, int ts, uint32_t& tile) {
-    while (unit == units) {
-      Seg s;
-      long long rs;
-      if (!next_seg(walk, p, s, rs)) return 0;
-      table = p.block_table + static_cast<size_t>(s.b) * p.max_blocks;
-      n = s.s1 - s.s0;
-      s0 = s.s0;
-      hg = s.hg;
-      unit = 0;
-      units = my_units(n, ts, p.pl.TS);
-      cur = look_up(p, 0, ts);
-      nxt = look_up(p, 16, ts);
-    }
-    const int i = unit & 15;
-    if (i == 0 && unit > 0) {
-      cur = nxt;
-      nxt = look_up(p, unit + 16, ts);
-    }
-    tile = __shfl_sync(kFull, cur, 2 * i + (threadIdx.x & 1));
-    const int c = min(2, n - 2 * (unit * p.pl.TS + ts));
-    ++unit;
-    return c;
-  }
-};
-
 // A warp's softmax state: lane (g, t) holds heads 2 t and 2 t + 1 (n = 0, 1):
 // the reference M, the weights' sum l and dims 32 y + 4 g + 2 u + v in
 // acc[2 y + u][2 v + n].
@@ -305,37 +274,31 @@ struct State {
 }  // namespace
 
 template <int NG>
-__global__ void __launch_bounds__(kMaxWarps * 32, 1)
+__global__ void __launch_bounds__(kThreads, 1)
     kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
   constexpr int kGroup = 128 / NG, kTile = tile_bytes(kGroup);
-  constexpr uint32_t kUnit = 2 * kTile;  // K (or V) of a unit
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ long long sh_warp[32];
   __shared__ long long sh_info[8];
-  __shared__ __align__(8) unsigned long long sh_bar[kMaxWarps][2][kMaxUnits];
-  __shared__ Walk sh_walk[kMaxWarps][2];
+  __shared__ __align__(8) unsigned long long sh_full[kMaxSlots], sh_empty[kMaxSlots];
+  __shared__ Walk sh_walk[kMaxWarps + 1];
 
   const Plan& pl = p.pl;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int g = lane >> 2, t = lane & 3;
-  const int team = warp / pl.TS, ts = warp - team * pl.TS;  // team = (kv head, q-head tile)
-  const int hl = team / pl.NT, j0 = (team - hl * pl.NT) * 8;
-  const int cnt = min(8, pl.G - j0);
-  float* const scratch = reinterpret_cast<float*>(smem + pl.warps * pl.units * 2 * kUnit) +
-                         static_cast<size_t>(team) * (pl.TS / 2) * kPassWords * 32;
+  const uint32_t ring = smem_u32(smem);
+  const uint32_t full = smem_u32(sh_full), empty = smem_u32(sh_empty);
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (lane == 0) {
-    for (int i = 0; i < pl.units; ++i) {
-      mbar_init(smem_u32(&sh_bar[warp][0][i]), 1);
-      mbar_init(smem_u32(&sh_bar[warp][1][i]), 1);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < pl.nslots; ++i) {
+      mbar_init(full + 8 * i, 1);
+      mbar_init(empty + 8 * i, pl.warps);
     }
     fence_mbar_init();
   }
   balanced_start(
       p.B, pl.NHG, [&](int b) -> long long { return tiles_of(req_len(p, b)); }, sh_warp, sh_info);
-  const long long E = sh_info[2], T = sh_info[5];
-  if (lane < 2) {
+  if (threadIdx.x <= kMaxWarps) {
     Walk w;
     w.g = sh_info[0];
     w.g_end = sh_info[1];
@@ -344,33 +307,74 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
     w.hg = 0;
     w.S = w.g < w.g_end ? req_len(p, w.b) : 0;
     w.L = tiles_of(w.S);
-    sh_walk[warp][lane] = w;
+    sh_walk[threadIdx.x] = w;
   }
-  __syncwarp();
+  __syncthreads();
+  Seg s;
+  long long row_start;
 
-  // ---- this warp's copies: unit u in slot u mod units, K and V apart ----
-  const uint32_t ring = smem_u32(smem) + static_cast<uint32_t>(warp * pl.units) * 2 * kUnit;
-  const uint32_t bar_k = smem_u32(&sh_bar[warp][0][0]), bar_v = smem_u32(&sh_bar[warp][1][0]);
-  const uint64_t pol = policy_evict_first();
-  Copier cp;
-  cp.unit = cp.units = 0;
-  const auto copy = [&](const unsigned char* cache, uint32_t tile, int hg, int c, uint32_t dst,
-                        uint32_t bar) {
-    if (lane == 0) mbar_arrive_expect_tx(bar, c * kTile);
-    __syncwarp();
-    if (lane < c)
-      bulk_g2s(dst + lane * kTile,
-               cache + (static_cast<size_t>(tile) * p.Hkv + hg * pl.HG + hl) * kTile, kTile, bar, pol);
-  };
-  int pending = 0;  // units copied and not yet done with
-  for (int i = 0; i < pl.units; ++i) {
-    uint32_t tile;
-    const int c = cp.next(p, &sh_walk[warp][0], ts, tile);
-    if (c == 0) break;
-    copy(p.k, tile, cp.hg, c, ring + i * 2 * kUnit, bar_k + 8 * i);
-    copy(p.v, tile, cp.hg, c, ring + i * 2 * kUnit + kUnit, bar_v + 8 * i);
-    ++pending;
+  if (warp >= kMaxWarps) {
+    // -------------------------------- copies --------------------------------
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCopyRegs));
+    if (warp > kMaxWarps) return;
+    const uint32_t row_bytes = static_cast<uint32_t>(pl.HG * kTile);
+    int slot = 0;
+    uint32_t phase = 0;
+    int issued = 0;  // slots filled, counted up to nslots
+    bool ok = true;
+    while (ok && next_seg(&sh_walk[kMaxWarps], p, s, row_start)) {
+      const int* table = p.block_table + static_cast<size_t>(s.b) * p.max_blocks;
+      for (int st = s.s0; st < s.s1 && ok; st += pl.slot_tiles) {
+        const int nt = min(pl.slot_tiles, s.s1 - st);
+        size_t off = 0;
+        if (lane < nt) {
+          const int lb = (st + lane) / p.tiles_per_block, sub = st + lane - lb * p.tiles_per_block;
+          int page = ld_nc_s32(table + lb);
+          if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_blocks)) {
+            raise_status(kStatusBadPage);
+            page = 0;
+          }
+          off = ((static_cast<size_t>(page) * p.tiles_per_block + sub) * p.Hkv +
+                 static_cast<size_t>(s.hg) * pl.HG) * kTile;
+        }
+        for (int kv = 0; kv < 2; ++kv) {
+          if (!__all_sync(kFull, mbar_wait(empty + 8 * slot, phase ^ 1))) {
+            raise_status(kStatusWaitTimeout);
+            ok = false;
+            break;
+          }
+          if (lane == 0) mbar_arrive_expect_tx(full + 8 * slot, row_bytes * nt);
+          __syncwarp();
+          if (lane < nt)
+            bulk_g2s(ring + slot * pl.slot_bytes + lane * row_bytes, (kv ? p.v : p.k) + off,
+                     row_bytes, full + 8 * slot, policy_evict_first());
+          issued = min(issued + 1, pl.nslots);
+          if (++slot == pl.nslots) {
+            slot = 0;
+            phase ^= 1;
+          }
+        }
+      }
+    }
+    // No copy may land after the CTA has exited: wait (each with its limit)
+    // for the last `issued` slots (see the K1 scan).
+    for (int j = 0; j < issued; ++j) {
+      if (--slot < 0) {
+        slot = pl.nslots - 1;
+        phase ^= 1;
+      }
+      mbar_wait(full + 8 * slot, phase);
+    }
+    return;
   }
+
+  // ------------------------------ consumers -------------------------------
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kConsumerRegs));
+  if (warp >= pl.warps) return;
+  const int g = lane >> 2, t = lane & 3;
+  const int team = warp / pl.TS, ts = warp - team * pl.TS;  // team = (kv head, q-head tile)
+  const int hl = team / pl.NT, j0 = (team - hl * pl.NT) * 8;
+  const int cnt = min(8, pl.G - j0);
 
   // Requests without tokens occupy no tiles: CTA (b mod grid) zeroes them.
   for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
@@ -386,160 +390,137 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
 
   int slot = 0;
   uint32_t phase = 0;
-  // After a wait gave up: waits (each with its limit) for the copies of the
-  // next nk units' K and nv units' V, so that none lands after the CTA's end.
-  const auto drain = [&](int nk, int nv) {
-    for (int k = 0; k < max(nk, nv); ++k) {
-      const bool wrap = slot + k >= pl.units;
-      const int sl = wrap ? slot + k - pl.units : slot + k;
-      const uint32_t ph = wrap ? phase ^ 1u : phase;
-      if (k < nk) mbar_wait(bar_k + 8 * sl, ph);
-      if (k < nv) mbar_wait(bar_v + 8 * sl, ph);
-    }
+  const auto advance = [&]() {  // this warp has read the slot
     __syncwarp();
+    if (lane == 0) mbar_arrive(empty + 8 * slot);
+    if (++slot == pl.nslots) {
+      slot = 0;
+      phase ^= 1;
+    }
   };
   bool dead = false;  // a wait gave up: empty states from here on (see the K1 scan)
   bool first_seg = true;
-  Seg s;
-  long long row_start;
-  while (next_seg(&sh_walk[warp][1], p, s, row_start)) {
+  while (next_seg(&sh_walk[warp], p, s, row_start)) {
+    const long long E = sh_info[2], T = sh_info[5];
     const long long row_end = row_start + tiles_of(s.S);
-    s.cfirst = range_owner(row_start, T, E);
-    s.nparts = static_cast<int>(range_owner(row_end - 1, T, E) - s.cfirst + 1);
+    const int cfirst = static_cast<int>(range_owner(row_start, T, E));
+    const int nparts = static_cast<int>(range_owner(row_end - 1, T, E)) - cfirst + 1;
     if (warp == 0 && lane == 0) {
-      if (first_seg && s.nparts > 1 && row_start + s.s1 == row_end)
-        p.ends[blockIdx.x] = make_int2(s.row, s.nparts);
-      if (s.s0 == 0) p.row_info[s.row] = make_int2(static_cast<int>(s.cfirst), s.nparts);
+      if (first_seg && nparts > 1 && row_start + s.s1 == row_end)
+        p.ends[blockIdx.x] = make_int2(s.row, nparts);
+      if (s.s0 == 0) p.row_info[s.row] = make_int2(cfirst, nparts);
     }
     first_seg = false;
     const int hbase = (s.hg * pl.HG + hl) * pl.G + j0;
-    const int units = my_units(s.s1 - s.s0, ts, pl.TS);
-    const int active = min(pl.TS, (s.s1 - s.s0 + 1) / 2);  // warps of the team with a unit
+
+    // q fragments (B operand): lane (g, t) holds head g, words 4 i + t, each
+    // as the dim pairs (0, 4), (1, 5), (2, 6), (3, 7) that meet the codes.
+    uint32_t qf[8][2];
+    uint32_t qc, qs;  // 2^-24 Q, and -8 2^-24 Q of the q that meets the codes
+    float fac[2];     // what takes a sum to the score in log2 units
+    {
+      const bool has = g < cnt;
+      const __nv_bfloat16* qrow =
+          p.q + (static_cast<size_t>(s.b) * p.Hq + hbase + (has ? g : 0)) * kHeadDim;
+      uint4 w[4];
+      uint32_t top = 0;  // largest |q| of the head, as bits
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = has ? __ldg(reinterpret_cast<const uint4*>(qrow + 8 * (4 * i + t)))
+                   : make_uint4(0, 0, 0, 0);
+        const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+        #pragma unroll
+        for (int k = 0; k < 4; ++k) top = max(top, max(u[k] & 0x7fffu, (u[k] >> 16) & 0x7fffu));
+      }
+      top = max(top, __shfl_xor_sync(kFull, top, 1));
+      top = max(top, __shfl_xor_sync(kFull, top, 2));
+      const int e = max(-100, min(100, static_cast<int>(top >> 7) - 127));
+      const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);  // 2^-e
+      const float up =
+          p.scale_log2 * 16777216.f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+      fac[0] = __shfl_sync(kFull, up, 8 * t);
+      fac[1] = __shfl_sync(kFull, up, 8 * t + 4);
+      float Q[NG], R[NG];  // sums of q, and of what the roundings leave of it
+      #pragma unroll
+      for (int y = 0; y < NG; ++y) Q[y] = R[y] = 0.f;
+      #pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+        float q[8];
+        #pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          q[2 * k] = __uint_as_float(u[k] << 16) * down;
+          q[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u) * down;
+        }
+        const float h = 0.0625f;
+        const __half d2 = __float2half_rn(q[2] - q[3] * h), d6 = __float2half_rn(q[6] - q[7] * h);
+        qf[2 * i][0] = pack_half2(q[0], q[4]);
+        qf[2 * i][1] = pack_half2(q[1] * h, q[5] * h);
+        qf[2 * i + 1][0] = pack_half2(__half2float(d2), __half2float(d6));
+        qf[2 * i + 1][1] = pack_half2(q[3] * h, q[7] * h);
+        const float rest = q[0] + q[4] + q[1] + q[5] + q[3] + q[7];
+        float a = rest + (q[2] + q[6]);
+        float b = rest + (__half2float(d2) + q[3] * h) + (__half2float(d6) + q[7] * h);
+        #pragma unroll
+        for (int off = 1; off < 4; off <<= 1) {
+          a += __shfl_xor_sync(kFull, a, off);
+          b += __shfl_xor_sync(kFull, b, off);
+        }
+        Q[i * NG / 4] += a;
+        R[i * NG / 4] += b;
+      }
+      #pragma unroll
+      for (int y = 0; y < NG; ++y) {
+        Q[y] *= 1.f / 16777216.f;
+        R[y] *= -8.f / 16777216.f;
+      }
+      qc = high_low<NG>(Q, t);
+      qs = high_low<NG>(R, t);
+    }
 
     State a;
     a.m[0] = a.m[1] = kNoRef;
     a.l[0] = a.l[1] = 0.f;
     #pragma unroll
     for (int mt = 0; mt < 8; ++mt) a.acc[mt][0] = a.acc[mt][1] = a.acc[mt][2] = a.acc[mt][3] = 0.f;
+    float cw[4] = {0.f, 0.f, 0.f, 0.f};  // sum_t p_t c_ty: row y = g, heads 2 t, 2 t + 1
 
-    if (units > 0) {
-      // q fragments (B operand): lane (g, t) holds head g, words 4 i + t, each
-      // as the dim pairs (0, 4), (1, 5), (2, 6), (3, 7) that meet the codes.
-      uint32_t qf[8][2];
-      uint32_t qsum_b;     // 2^-24 Q, high and low bf16 parts, as a B operand
-      float start[NG][2];  // -8 2^-24 Q of heads 2 t, 2 t + 1
-      float fac[2];        // what takes a sum to the score in log2 units
-      {
-        const bool has = g < cnt;
-        const __nv_bfloat16* qrow =
-            p.q + (static_cast<size_t>(s.b) * p.Hq + hbase + (has ? g : 0)) * kHeadDim;
-        uint4 w[4];
-        uint32_t top = 0;  // largest |q| of the head, as bits
-        #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          w[i] = has ? __ldg(reinterpret_cast<const uint4*>(qrow + 8 * (4 * i + t)))
-                     : make_uint4(0, 0, 0, 0);
-          const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-          #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            top = max(top, max(u[k] & 0x7fffu, (u[k] >> 16) & 0x7fffu));
-        }
-        top = max(top, __shfl_xor_sync(kFull, top, 1));
-        top = max(top, __shfl_xor_sync(kFull, top, 2));
-        const int e = max(-100, min(100, static_cast<int>(top >> 7) - 127));
-        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);  // 2^-e
-        const float up = p.scale_log2 * 16777216.f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-        fac[0] = __shfl_sync(kFull, up, 8 * t);
-        fac[1] = __shfl_sync(kFull, up, 8 * t + 4);
-        float Q[NG];
-        #pragma unroll
-        for (int y = 0; y < NG; ++y) Q[y] = 0.f;
-        #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-          float q[8];
-          float sum = 0.f;
-          #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            q[2 * k] = __uint_as_float(u[k] << 16) * down;
-            q[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u) * down;
-          }
-          #pragma unroll
-          for (int k = 0; k < 8; ++k) sum += q[k];
-          qf[2 * i][0] = pack_half2(q[0], q[4]);
-          qf[2 * i][1] = pack_half2(q[1] * 0.0625f, q[5] * 0.0625f);
-          qf[2 * i + 1][0] = pack_half2(q[2], q[6]);
-          qf[2 * i + 1][1] = pack_half2(q[3] * 0.0625f, q[7] * 0.0625f);
-          sum += __shfl_xor_sync(kFull, sum, 1);
-          sum += __shfl_xor_sync(kFull, sum, 2);
-          Q[i * NG / 4] += sum;
-        }
-        float hi[NG], lo[NG];
-        #pragma unroll
-        for (int y = 0; y < NG; ++y) {
-          Q[y] *= 1.f / 16777216.f;
-          start[y][0] = -8.f * __shfl_sync(kFull, Q[y], 8 * t);
-          start[y][1] = -8.f * __shfl_sync(kFull, Q[y], 8 * t + 4);
-          hi[y] = __bfloat162float(__float2bfloat16(Q[y]));
-          lo[y] = Q[y] - hi[y];
-        }
-        if constexpr (NG == 4) {
-          const uint32_t h01 = pack_bf16x2(hi[0], hi[1]), h23 = pack_bf16x2(hi[2], hi[3]);
-          const uint32_t l01 = pack_bf16x2(lo[0], lo[1]), l23 = pack_bf16x2(lo[2], lo[3]);
-          qsum_b = t < 2 ? (t == 0 ? h01 : h23) : (t == 2 ? l01 : l23);
-        } else if constexpr (NG == 2) {
-          qsum_b = t == 0 ? pack_bf16x2(hi[0], hi[1]) : (t == 1 ? pack_bf16x2(lo[0], lo[1]) : 0u);
-        } else {
-          qsum_b = t == 0 ? pack_bf16x2(hi[0], lo[0]) : 0u;
-        }
+    for (int st = s.s0 + 2 * ts; st - 2 * ts < s.s1; st += pl.slot_tiles) {
+      const bool work = st < s.s1;
+      const int left = min(s.S - st * kTileTokens, (s.s1 - st) * kTileTokens);  // tokens from here on
+      const uint32_t tile0 = ring + slot * pl.slot_bytes + (2 * ts * pl.HG + hl) * kTile;
+      const uint32_t tile_step = static_cast<uint32_t>(pl.HG * kTile);
+      float x[2][4];
+
+      // ---- scores of two tiles ----
+      if (!__all_sync(kFull, mbar_wait(full + 8 * slot, phase))) {
+        dead = true;
+        break;
       }
-      float cw[4] = {0.f, 0.f, 0.f, 0.f};  // sum_t p_t c_ty: row y = g, heads 2 t, 2 t + 1
-
-      for (int i = 0; i < units && !dead; ++i) {
-        const int tile_no = s.s0 + 2 * (i * pl.TS + ts);
-        const int left = s.S - tile_no * kTileTokens;  // valid tokens from here on
-        const bool two = tile_no + 1 < s.s1;
-        const uint32_t kb = ring + static_cast<uint32_t>(slot) * 2 * kUnit, vb = kb + kUnit;
-        float x[2][4];
-
-        // ---- scores of two tiles ----
-        if (!__all_sync(kFull, mbar_wait(bar_k + 8 * slot, phase))) {
-          drain(pending, pending);
-          dead = true;
-          break;
-        }
+      if (work) {
         #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          // (a unit without a second tile reads what the slot held before; its
+          // (without a second tile this reads what the slot held before; its
           // scores are masked like those behind the last token)
-          const uint32_t tb = kb + j * kTile;
+          const uint32_t tb = tile0 + j * tile_step;
           const uint4 wa = lds128(tb + 64 * g + 16 * t), wb = lds128(tb + 512 + 64 * g + 16 * t);
           const uint32_t ua[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
-          float sa[NG], sb[NG];
-          load_scales<NG>(tb + scale_at(0, 0, NG) + 2 * NG * g, sa);
-          load_scales<NG>(tb + scale_at(8, 0, NG) + 2 * NG * g, sb);
-          uint32_t ca, cb;
-          if constexpr (NG == 4) {
-            ca = lds32(tb + k_centre_at(0, 0, NG) + 8 * g + 4 * (t & 1));
-            cb = lds32(tb + k_centre_at(8, 0, NG) + 8 * g + 4 * (t & 1));
-          } else if constexpr (NG == 2) {
-            ca = lds32(tb + k_centre_at(0, 0, NG) + 4 * g);
-            cb = lds32(tb + k_centre_at(8, 0, NG) + 4 * g);
-          } else {
-            ca = lds16(tb + k_centre_at(0, 0, NG) + 2 * g) * 0x10001u;
-            cb = lds16(tb + k_centre_at(8, 0, NG) + 2 * g) * 0x10001u;
-          }
+          Scales<NG> sa, sb, ca, cb;
+          sa.load(tb + scale_at(0, 0, NG) + 2 * NG * g);
+          sb.load(tb + scale_at(8, 0, NG) + 2 * NG * g);
+          ca.load(tb + k_centre_at(0, 0, NG) + 2 * NG * g);
+          cb.load(tb + k_centre_at(8, 0, NG) + 2 * NG * g);
           float sc[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_bf16_16816(sc, ca, cb, 0u, 0u, qsum_b, 0u);
+          mma_bf16_16816(sc, ca.operand(t), cb.operand(t), sa.operand(t), sb.operand(t), qc, qs);
           #pragma unroll
           for (int y = 0; y < NG; ++y) {
-            float d[4] = {start[y][0], start[y][1], start[y][0], start[y][1]};
+            float d[4] = {0.f, 0.f, 0.f, 0.f};
             #pragma unroll
             for (int k = y * (4 / NG); k < (y + 1) * (4 / NG); ++k) {
-              mma_f16_16816(d, low_codes(ua[k]), low_codes(ub[k]), high_codes(ua[k]),
-                            high_codes(ub[k]), qf[2 * k][0], qf[2 * k][1]);
-              mma_f16_16816(d, low_codes(ua[k] >> 8), low_codes(ub[k] >> 8), high_codes(ua[k] >> 8),
-                            high_codes(ub[k] >> 8), qf[2 * k + 1][0], qf[2 * k + 1][1]);
+              mma_f16_16816(d, codes_n(ua[k]), codes_n(ub[k]), codes_16n(ua[k]), codes_16n(ub[k]),
+                            qf[2 * k][0], qf[2 * k][1]);
+              const uint32_t ba = codes_byte(ua[k]), bb = codes_byte(ub[k]);
+              mma_f16_16816(d, codes_n(ba), codes_n(bb), ba, bb, qf[2 * k + 1][0], qf[2 * k + 1][1]);
             }
             sc[0] += sa[y] * d[0];
             sc[1] += sa[y] * d[1];
@@ -549,63 +530,63 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
           #pragma unroll
           for (int k = 0; k < 4; ++k) x[j][k] = sc[k] * fac[k & 1];
         }
-        if (left < 2 * kTileTokens || !two) {
-          const int nv = two ? left : min(left, kTileTokens);
+        if (left < 2 * kTileTokens) {
           #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            if (j * kTileTokens + g >= nv) x[j][0] = x[j][1] = -INFINITY;
-            if (j * kTileTokens + g + 8 >= nv) x[j][2] = x[j][3] = -INFINITY;
+            if (j * kTileTokens + g >= left) x[j][0] = x[j][1] = -INFINITY;
+            if (j * kTileTokens + g + 8 >= left) x[j][2] = x[j][3] = -INFINITY;
           }
         }
-        __syncwarp();  // every lane has read the K slot: refill it
-        uint32_t next_tile;
-        const int next_c = cp.next(p, &sh_walk[warp][0], ts, next_tile);
-        if (next_c) copy(p.k, next_tile, cp.hg, next_c, kb, bar_k + 8 * slot);
+      }
+      advance();
 
-        // ---- weights, and the sum over V ----
-        if (!__all_sync(kFull, mbar_wait(bar_v + 8 * slot, phase))) {
-          drain(pending + (next_c ? 1 : 0), pending);
-          dead = true;
-          break;
-        }
+      // ---- weights, and the sum over V ----
+      const uint32_t vb = ring + slot * pl.slot_bytes + (2 * ts * pl.HG + hl) * kTile;
+      if (!__all_sync(kFull, mbar_wait(full + 8 * slot, phase))) {
+        dead = true;
+        break;
+      }
+      if (work) {
         uint32_t pw[2][2], bw[2][2][NG];  // weights (bf16), and times the scales (fp16)
         #pragma unroll 1
         for (int pass = 0;; ++pass) {
           float sm = 0.f;
           uint32_t over = 0u;  // largest fp16 weight
-          float l[2] = {0.f, 0.f}, w[2][4];
+          float l[2] = {0.f, 0.f};
           #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float sa[NG], sb[NG];
-            load_scales<NG>(vb + j * kTile + scale_at(0, 0, NG) + 2 * NG * g, sa);
-            load_scales<NG>(vb + j * kTile + scale_at(8, 0, NG) + 2 * NG * g, sb);
-            if (left < 2 * kTileTokens || !two) {
+            const uint32_t tb = vb + j * tile_step;
+            Scales<NG> sa, sb;
+            sa.load(tb + scale_at(0, 0, NG) + 2 * NG * g);
+            sb.load(tb + scale_at(8, 0, NG) + 2 * NG * g);
+            if (left < 2 * kTileTokens) {
               // what lies behind the last token may be anything
-              const int nv = two ? left : min(left, kTileTokens);
               #pragma unroll
-              for (int y = 0; y < NG; ++y) {
-                if (j * kTileTokens + g >= nv) sa[y] = 0.f;
-                if (j * kTileTokens + g + 8 >= nv) sb[y] = 0.f;
+              for (int k = 0; k < (NG + 1) / 2; ++k) {
+                if (j * kTileTokens + g >= left) sa.w[k] = 0u;
+                if (j * kTileTokens + g + 8 >= left) sb.w[k] = 0u;
               }
             }
+            float w[4];
             #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              w[j][k] = exp2_approx(x[j][k] - a.m[k & 1]);
-              l[k & 1] += w[j][k];
+              w[k] = exp2_approx(x[j][k] - a.m[k & 1]);
+              l[k & 1] += w[k];
             }
-            pw[j][0] = pack_bf16x2(w[j][0], w[j][1]);
-            pw[j][1] = pack_bf16x2(w[j][2], w[j][3]);
+            pw[j][0] = pack_bf16x2(w[0], w[1]);
+            pw[j][1] = pack_bf16x2(w[2], w[3]);
             #pragma unroll
             for (int y = 0; y < NG; ++y) {
-              sm = fmaxf(sm, fmaxf(sa[y], sb[y]));
-              bw[j][0][y] = pack_half2(w[j][0] * sa[y], w[j][1] * sa[y]);
-              bw[j][1][y] = pack_half2(w[j][2] * sb[y], w[j][3] * sb[y]);
+              const float fa = sa[y], fb = sb[y];
+              sm = fmaxf(sm, fmaxf(fa, fb));
+              bw[j][0][y] = pack_half2(w[0] * fa, w[1] * fa);
+              bw[j][1][y] = pack_half2(w[2] * fb, w[3] * fb);
               over = max_half2(over, max_half2(bw[j][0][y], bw[j][1][y]));
             }
           }
           // 2^15 in either half, or a weight sum that nears fp32's range
-          const bool big = (over & 0xffffu) >= 0x7800u || over >= 0x78000000u ||
-                           l[0] > 1e30f || l[1] > 1e30f;
+          const bool big = (over & 0xffffu) >= 0x7800u || over >= 0x78000000u || l[0] > 1e30f ||
+                           l[1] > 1e30f;
           if (pass == 1 || !__any_sync(kFull, big)) {
             a.l[0] += l[0];
             a.l[1] += l[1];
@@ -633,8 +614,9 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
         }
         #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          if (j == 1 && !two) break;
-          const uint32_t tb = vb + j * kTile;
+          const int nv = left - j * kTileTokens;
+          if (j == 1 && nv <= 0) break;
+          const uint32_t tb = vb + j * tile_step;
           const uint32_t va = tb + 128 * t + 16 * (g ^ (2 * t));
           const uint4 wa = lds128(va), wb = lds128(va + 512);
           const uint32_t ua[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
@@ -643,7 +625,6 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
             ca = lds32(tb + v_centre_at(0, 0, NG) + 32 * g + 4 * t);
             cb = lds32(tb + v_centre_at(8, 0, NG) + 32 * g + 4 * t);
           }
-          const int nv = left - j * kTileTokens;
           if (nv < kTileTokens) {
             if (2 * t >= nv) ca = 0u; else if (2 * t + 1 >= nv) ca &= 0xffffu;
             if (2 * t + 8 >= nv) cb = 0u; else if (2 * t + 9 >= nv) cb &= 0xffffu;
@@ -654,51 +635,55 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
             const uint32_t b0 = movmatrix_trans(bw[j][0][y]), b1 = movmatrix_trans(bw[j][1][y]);
             #pragma unroll
             for (int k = y * (4 / NG); k < (y + 1) * (4 / NG); ++k) {
-              mma_f16_16816(a.acc[2 * k], low_centred(ua[k]), high_centred(ua[k]),
-                            low_centred(ub[k]), high_centred(ub[k]), b0, b1);
-              mma_f16_16816(a.acc[2 * k + 1], low_centred(ua[k] >> 8), high_centred(ua[k] >> 8),
-                            low_centred(ub[k] >> 8), high_centred(ub[k] >> 8), b0, b1);
+              mma_f16_16816(a.acc[2 * k], sub_half2(codes_n(ua[k]), 0x00080008u),
+                            sub_half2(codes_16n(ua[k]), 0x00800080u),
+                            sub_half2(codes_n(ub[k]), 0x00080008u),
+                            sub_half2(codes_16n(ub[k]), 0x00800080u), b0, b1);
+              const uint32_t ba = codes_byte(ua[k]), bb = codes_byte(ub[k]);
+              mma_f16_16816(a.acc[2 * k + 1], sub_half2(codes_n(ba), 0x00080008u),
+                            sub_half2(ba, 0x00880088u), sub_half2(codes_n(bb), 0x00080008u),
+                            sub_half2(bb, 0x00880088u), b0, b1);
             }
           }
         }
-        __syncwarp();  // every lane has read the V slot
-        if (next_c) copy(p.v, next_tile, cp.hg, next_c, vb, bar_v + 8 * slot);
-        else --pending;
-        if (++slot == pl.units) {
-          slot = 0;
-          phase ^= 1;
-        }
       }
-
-      // ---- the warp's own sums ----
-      #pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) a.l[n] += __shfl_xor_sync(kFull, a.l[n], off);
-        #pragma unroll
-        for (int y = 0; y < NG; ++y) {
-          const float c = __shfl_sync(kFull, cw[n], 4 * y + t);
-          #pragma unroll
-          for (int k = y * (4 / NG); k < (y + 1) * (4 / NG); ++k)
-            #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              a.acc[2 * k + u][n] += c;
-              a.acc[2 * k + u][2 + n] += c;
-            }
-        }
-      }
+      advance();
     }
+
+    // ---- segment epilogue: the warp's own sums, in full units ----
     if (dead) {
       if (lane == 0) raise_status(kStatusWaitTimeout);
       a.m[0] = a.m[1] = -INFINITY;
       a.l[0] = a.l[1] = 0.f;
+      cw[0] = cw[1] = 0.f;
       #pragma unroll
       for (int mt = 0; mt < 8; ++mt)
         a.acc[mt][0] = a.acc[mt][1] = a.acc[mt][2] = a.acc[mt][3] = 0.f;
     }
+    #pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      #pragma unroll
+      for (int off = 4; off < 32; off <<= 1) a.l[n] += __shfl_xor_sync(kFull, a.l[n], off);
+      #pragma unroll
+      for (int y = 0; y < NG; ++y) {
+        const float c = __shfl_sync(kFull, cw[n], 4 * y + t);
+        #pragma unroll
+        for (int k = y * (4 / NG); k < (y + 1) * (4 / NG); ++k) {
+          float(&e)[4] = a.acc[2 * k];
+          float(&o)[4] = a.acc[2 * k + 1];
+          o[2 + n] = (o[2 + n] - o[n]) * 1048576.f + c;  // a byte's 16 out' + out
+          o[n] = o[n] * 16777216.f + c;
+          e[2 + n] = e[2 + n] * 1048576.f + c;
+          e[n] = e[n] * 16777216.f + c;
+        }
+      }
+    }
 
     // ---- the team meets: halves hand over to halves, a few words at a time ----
+    const int active = min(pl.TS, (s.s1 - s.s0 + 1) / 2);  // warps of the team with tiles
     if (active > 1) {
+      float* const scratch = reinterpret_cast<float*>(smem + pl.nslots * pl.slot_bytes) +
+                             team * (pl.TS / 2) * kPassWords * 32;
       for (int off = pl.TS / 2; off >= 1; off >>= 1) {
         if (off >= active) continue;  // uniform over the team
         const bool gives = ts >= off && ts < 2 * off && ts < active;
@@ -748,7 +733,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
     for (int n = 0; n < 2; ++n) {
       const int head = 2 * t + n;
       if (head >= cnt) continue;
-      if (s.nparts == 1) {
+      if (nparts == 1) {
         __nv_bfloat16* o = p.out + (static_cast<size_t>(s.b) * p.Hq + hbase + head) * kHeadDim + 4 * g;
         const float inv = 1.f / a.l[n];
         #pragma unroll
@@ -757,7 +742,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32, 1)
               make_uint2(pack_bf16x2(a.acc[2 * y][n] * inv, a.acc[2 * y][2 + n] * inv),
                          pack_bf16x2(a.acc[2 * y + 1][n] * inv, a.acc[2 * y + 1][2 + n] * inv));
       } else {
-        // slot of the partial state: this CTA's, of the row's (K1's layout)
+        // this CTA's slot of the row (K1's layout)
         const size_t idx = (static_cast<size_t>(blockIdx.x) + s.row) * (pl.HG * pl.G) + hl * pl.G +
                            j0 + head;
         if (g == 0) {
@@ -863,10 +848,11 @@ int make_plan(int Hq, int Hkv, int group, Plan* p) {
   p->TS = 1;
   while (2 * p->TS * p->HG * p->NT <= kMaxWarps) p->TS *= 2;
   p->warps = p->HG * p->NT * p->TS;
-  const int unit_bytes = 4 * tile_bytes(group);  // K and V of two tiles
+  p->slot_tiles = 2 * p->TS;
+  p->slot_bytes = p->slot_tiles * p->HG * tile_bytes(group);
   const int scratch = p->HG * p->NT * (p->TS / 2) * kPassWords * 32 * 4;
-  p->units = std::min(kMaxUnits, (kSmemLimit - kSmemStatic - scratch) / (p->warps * unit_bytes));
-  p->smem = p->warps * p->units * unit_bytes + scratch;
+  p->nslots = std::min(kMaxSlots, (kSmemLimit - kSmemStatic - scratch) / p->slot_bytes);
+  p->smem = p->nslots * p->slot_bytes + scratch;
   return 0;
 }
 
@@ -967,7 +953,7 @@ cudaError_t kv4_decode_launch(const gqa_bf16* q, const unsigned char* k_cache,
   p.num_blocks = num_blocks;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.pl = pl;
-  const int threads = pl.warps * 32;
+  const int threads = kThreads;
   if (group == 32) kv4_decode_kernel<4><<<grid, threads, pl.smem, stream>>>(p);
   else if (group == 64) kv4_decode_kernel<2><<<grid, threads, pl.smem, stream>>>(p);
   else kv4_decode_kernel<1><<<grid, threads, pl.smem, stream>>>(p);
