@@ -95,22 +95,16 @@ struct DecodeParams {
   Plan pl;
 };
 
-__device__ __forceinline__ uint4 lds128(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "r"(a));
-  return v;
+// Shared-memory loads (plain ones: ordered by the waits' memory clobbers,
+// free to move between them).
+__device__ __forceinline__ uint4 lds128(const unsigned char* a) {
+  return *reinterpret_cast<const uint4*>(a);
 }
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
-  return v;
+__device__ __forceinline__ uint32_t lds32(const unsigned char* a) {
+  return *reinterpret_cast<const uint32_t*>(a);
 }
-__device__ __forceinline__ uint32_t lds16(uint32_t a) {
-  unsigned short v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(a));
-  return v;
+__device__ __forceinline__ uint32_t lds16(const unsigned char* a) {
+  return *reinterpret_cast<const unsigned short*>(a);
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -145,27 +139,48 @@ __device__ __forceinline__ uint32_t max_half2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// D = A(16x16, row) * B(16x8, col) + D, fp16 inputs, fp32 accumulators.
-__device__ __forceinline__ void mma_f16_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                              uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
-      "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+// D = A(16x16, row) * B(16x8, col) + C, fp32 sums of fp16 or bf16 products.
+// Not volatile: the operands say all that orders them.
+#define KV4_MMA(name, type)                                                                     \
+  __device__ __forceinline__ void name(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,    \
+                                       uint32_t a3, uint32_t b0, uint32_t b1) {                 \
+    asm("mma.sync.aligned.m16n8k16.row.col.f32." type "." type ".f32 "                          \
+        "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"                       \
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])                                        \
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));                                \
+  }                                                                                             \
+  __device__ __forceinline__ void name##_first(float (&d)[4], uint32_t a0, uint32_t a1,         \
+                                               uint32_t a2, uint32_t a3, uint32_t b0,           \
+                                               uint32_t b1) {                                   \
+    asm("mma.sync.aligned.m16n8k16.row.col.f32." type "." type ".f32 "                          \
+        "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"                   \
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])                                        \
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));                      \
+  }
+KV4_MMA(mma_f16, "f16")
+KV4_MMA(mma_bf16, "bf16")
+#undef KV4_MMA
+
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 // The NG bf16 scales (or centres) of one token, as stored: words of two.
 template <int NG>
 struct Scales {
   uint32_t w[(NG + 1) / 2];
-  __device__ __forceinline__ void load(uint32_t a) {
-    if constexpr (NG == 4)
-      asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a));
-    else if constexpr (NG == 2)
+  __device__ __forceinline__ void load(const unsigned char* a) {
+    if constexpr (NG == 4) {
+      const uint2 v = *reinterpret_cast<const uint2*>(a);
+      w[0] = v.x;
+      w[1] = v.y;
+    } else if constexpr (NG == 2) {
       w[0] = lds32(a);
-    else
+    } else {
       w[0] = lds16(a) * 0x10001u;
+    }
   }
   __device__ __forceinline__ float operator[](int y) const {
     return __uint_as_float(y & 1 ? w[y / 2] & 0xffff0000u : w[y / 2] << 16);
@@ -485,11 +500,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int mt = 0; mt < 8; ++mt) a.acc[mt][0] = a.acc[mt][1] = a.acc[mt][2] = a.acc[mt][3] = 0.f;
     float cw[4] = {0.f, 0.f, 0.f, 0.f};  // sum_t p_t c_ty: row y = g, heads 2 t, 2 t + 1
 
-    for (int st = s.s0 + 2 * ts; st - 2 * ts < s.s1; st += pl.slot_tiles) {
-      const bool work = st < s.s1;
-      const int left = min(s.S - st * kTileTokens, (s.s1 - st) * kTileTokens);  // tokens from here on
-      const uint32_t tile0 = ring + slot * pl.slot_bytes + (2 * ts * pl.HG + hl) * kTile;
-      const uint32_t tile_step = static_cast<uint32_t>(pl.HG * kTile);
+    // Tokens of the segment from this warp's next tile on; the team's warps take
+    // the chunks' pairs of tiles in turn, and all pass every chunk.
+    int left = min(s.S - s.s0 * kTileTokens, (s.s1 - s.s0) * kTileTokens) - 2 * ts * kTileTokens;
+    for (int chunks = (s.s1 - s.s0 + pl.slot_tiles - 1) / pl.slot_tiles; chunks > 0;
+         --chunks, left -= pl.slot_tiles * kTileTokens) {
+      const bool work = left > 0;
+      const unsigned char* kb = smem + slot * pl.slot_bytes + (2 * ts * pl.HG + hl) * kTile;
+      const int tile_step = pl.HG * kTile;
       float x[2][4];
 
       // ---- scores of two tiles ----
@@ -502,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < 2; ++j) {
           // (without a second tile this reads what the slot held before; its
           // scores are masked like those behind the last token)
-          const uint32_t tb = tile0 + j * tile_step;
+          const unsigned char* tb = kb + j * tile_step;
           const uint4 wa = lds128(tb + 64 * g + 16 * t), wb = lds128(tb + 512 + 64 * g + 16 * t);
           const uint32_t ua[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
           Scales<NG> sa, sb, ca, cb;
@@ -510,17 +528,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           sb.load(tb + scale_at(8, 0, NG) + 2 * NG * g);
           ca.load(tb + k_centre_at(0, 0, NG) + 2 * NG * g);
           cb.load(tb + k_centre_at(8, 0, NG) + 2 * NG * g);
-          float sc[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_bf16_16816(sc, ca.operand(t), cb.operand(t), sa.operand(t), sb.operand(t), qc, qs);
+          float sc[4];
+          mma_bf16_first(sc, ca.operand(t), cb.operand(t), sa.operand(t), sb.operand(t), qc, qs);
           #pragma unroll
           for (int y = 0; y < NG; ++y) {
-            float d[4] = {0.f, 0.f, 0.f, 0.f};
+            float d[4];
             #pragma unroll
             for (int k = y * (4 / NG); k < (y + 1) * (4 / NG); ++k) {
-              mma_f16_16816(d, codes_n(ua[k]), codes_n(ub[k]), codes_16n(ua[k]), codes_16n(ub[k]),
-                            qf[2 * k][0], qf[2 * k][1]);
               const uint32_t ba = codes_byte(ua[k]), bb = codes_byte(ub[k]);
-              mma_f16_16816(d, codes_n(ba), codes_n(bb), ba, bb, qf[2 * k + 1][0], qf[2 * k + 1][1]);
+              if (k == y * (4 / NG))
+                mma_f16_first(d, codes_n(ua[k]), codes_n(ub[k]), codes_16n(ua[k]), codes_16n(ub[k]),
+                              qf[2 * k][0], qf[2 * k][1]);
+              else
+                mma_f16(d, codes_n(ua[k]), codes_n(ub[k]), codes_16n(ua[k]), codes_16n(ub[k]),
+                        qf[2 * k][0], qf[2 * k][1]);
+              mma_f16(d, codes_n(ba), codes_n(bb), ba, bb, qf[2 * k + 1][0], qf[2 * k + 1][1]);
             }
             sc[0] += sa[y] * d[0];
             sc[1] += sa[y] * d[1];
@@ -541,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       advance();
 
       // ---- weights, and the sum over V ----
-      const uint32_t vb = ring + slot * pl.slot_bytes + (2 * ts * pl.HG + hl) * kTile;
+      const unsigned char* vb = smem + slot * pl.slot_bytes + (2 * ts * pl.HG + hl) * kTile;
       if (!__all_sync(kFull, mbar_wait(full + 8 * slot, phase))) {
         dead = true;
         break;
@@ -550,12 +572,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t pw[2][2], bw[2][2][NG];  // weights (bf16), and times the scales (fp16)
         #pragma unroll 1
         for (int pass = 0;; ++pass) {
-          float sm = 0.f;
           uint32_t over = 0u;  // largest fp16 weight
           float l[2] = {0.f, 0.f};
           #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const uint32_t tb = vb + j * tile_step;
+            const unsigned char* tb = vb + j * tile_step;
             Scales<NG> sa, sb;
             sa.load(tb + scale_at(0, 0, NG) + 2 * NG * g);
             sb.load(tb + scale_at(8, 0, NG) + 2 * NG * g);
@@ -578,7 +599,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             #pragma unroll
             for (int y = 0; y < NG; ++y) {
               const float fa = sa[y], fb = sb[y];
-              sm = fmaxf(sm, fmaxf(fa, fb));
               bw[j][0][y] = pack_half2(w[0] * fa, w[1] * fa);
               bw[j][1][y] = pack_half2(w[2] * fb, w[3] * fb);
               over = max_half2(over, max_half2(bw[j][0][y], bw[j][1][y]));
@@ -591,6 +611,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             a.l[0] += l[0];
             a.l[1] += l[1];
             break;
+          }
+          float sm = 0.f;  // largest scale of a token that counts
+          #pragma unroll 1
+          for (int i = g; i < min(left, 2 * kTileTokens); i += 8) {
+            Scales<NG> sc;
+            sc.load(vb + (i / kTileTokens) * tile_step + scale_at(i % kTileTokens, 0, NG));
+            #pragma unroll
+            for (int y = 0; y < NG; ++y) sm = fmaxf(sm, sc[y]);
           }
           #pragma unroll
           for (int off = 4; off < 32; off <<= 1) sm = fmaxf(sm, __shfl_xor_sync(kFull, sm, off));
@@ -616,8 +644,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j < 2; ++j) {
           const int nv = left - j * kTileTokens;
           if (j == 1 && nv <= 0) break;
-          const uint32_t tb = vb + j * tile_step;
-          const uint32_t va = tb + 128 * t + 16 * (g ^ (2 * t));
+          const unsigned char* tb = vb + j * tile_step;
+          const unsigned char* va = tb + 128 * t + 16 * (g ^ (2 * t));
           const uint4 wa = lds128(va), wb = lds128(va + 512);
           const uint32_t ua[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
           uint32_t ca = 0u, cb = 0u;
@@ -629,18 +657,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (2 * t >= nv) ca = 0u; else if (2 * t + 1 >= nv) ca &= 0xffffu;
             if (2 * t + 8 >= nv) cb = 0u; else if (2 * t + 9 >= nv) cb &= 0xffffu;
           }
-          mma_bf16_16816(cw, ca, 0u, cb, 0u, movmatrix_trans(pw[j][0]), movmatrix_trans(pw[j][1]));
+          mma_bf16(cw, ca, 0u, cb, 0u, transpose8x8(pw[j][0]), transpose8x8(pw[j][1]));
           #pragma unroll
           for (int y = 0; y < NG; ++y) {
-            const uint32_t b0 = movmatrix_trans(bw[j][0][y]), b1 = movmatrix_trans(bw[j][1][y]);
+            const uint32_t b0 = transpose8x8(bw[j][0][y]), b1 = transpose8x8(bw[j][1][y]);
             #pragma unroll
             for (int k = y * (4 / NG); k < (y + 1) * (4 / NG); ++k) {
-              mma_f16_16816(a.acc[2 * k], sub_half2(codes_n(ua[k]), 0x00080008u),
+              mma_f16(a.acc[2 * k], sub_half2(codes_n(ua[k]), 0x00080008u),
                             sub_half2(codes_16n(ua[k]), 0x00800080u),
                             sub_half2(codes_n(ub[k]), 0x00080008u),
                             sub_half2(codes_16n(ub[k]), 0x00800080u), b0, b1);
               const uint32_t ba = codes_byte(ua[k]), bb = codes_byte(ub[k]);
-              mma_f16_16816(a.acc[2 * k + 1], sub_half2(codes_n(ba), 0x00080008u),
+              mma_f16(a.acc[2 * k + 1], sub_half2(codes_n(ba), 0x00080008u),
                             sub_half2(ba, 0x00880088u), sub_half2(codes_n(bb), 0x00080008u),
                             sub_half2(bb, 0x00880088u), b0, b1);
             }
