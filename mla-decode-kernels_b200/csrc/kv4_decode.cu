@@ -17,11 +17,12 @@
 //     rounds (2^-12).  A q element below 2^-17 of its head's largest loses
 //     bits, 2^-25 of that largest at most.  The offset 8 is taken off by the
 //     centres' product, as the centre -8 s.
-//   * V: the same three patterns less 8, 128 and 136 (one packed subtraction,
-//     exact), so that the sums stay small: left positive they would pile up
-//     what the centres take away again, and over a long context fp32 loses
-//     the difference.  The byte's sum is 16 out' + out; the head's end
-//     resolves it.  The weights p_t s_ty are rounded to fp16, 2^-11.
+//   * V: the same patterns, again raw; a byte's sum is 16 out' + out, which
+//     the end resolves.  The offset 8 joins the centres, through one product
+//     of the weights with a constant.  The raw sums grow with the context
+//     while what remains of them need not, and fp32 would lose the difference,
+//     so every kFold pairs of tiles the centres' sum is folded into them.
+//     The weights p_t s_ty are rounded to fp16, 2^-11.
 // The softmax reference M of a head is no running maximum but any value that
 // keeps the fp16 weights in range: it is set so that the largest p s is 2^9
 // and moves only when one passes 2^15, so the common step takes no maximum
@@ -40,6 +41,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 #include <climits>
 #include <cstdint>
 
@@ -69,6 +71,7 @@ constexpr int kSmemLimit = 227 * 1024;
 constexpr int kSmemStatic = 3 * 1024;        // bound of the kernel's static shared memory
 constexpr int kPassWords = 8;                // floats per lane handed over at once at a meeting
 constexpr float kNoRef = -1e30f;             // M before the first token
+constexpr int kFold = 16;                    // pairs of tiles between two folds of the V sums
 
 __device__ __forceinline__ void raise_status(int bits) { atomicOr(&g_kv4_status, bits); }
 
@@ -119,13 +122,6 @@ __device__ __forceinline__ float exp2_approx(float x) {
 __device__ __forceinline__ uint32_t codes_n(uint32_t w) { return w & 0x000f000fu; }
 __device__ __forceinline__ uint32_t codes_16n(uint32_t w) { return w & 0x00f000f0u; }
 __device__ __forceinline__ uint32_t codes_byte(uint32_t w) { return __byte_perm(w, 0u, 0x4341); }
-
-// a - b in fp16 (exact here: multiples of 2^-24 below 2^-16).
-__device__ __forceinline__ uint32_t sub_half2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
 
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   uint32_t r;
@@ -498,28 +494,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     a.l[0] = a.l[1] = 0.f;
     #pragma unroll
     for (int mt = 0; mt < 8; ++mt) a.acc[mt][0] = a.acc[mt][1] = a.acc[mt][2] = a.acc[mt][3] = 0.f;
-    float cw[4] = {0.f, 0.f, 0.f, 0.f};  // sum_t p_t c_ty: row y = g, heads 2 t, 2 t + 1
+    // sum_t p_t (c_ty - 8 s_ty): row y = g, heads 2 t, 2 t + 1
+    float cw[4] = {0.f, 0.f, 0.f, 0.f};
 
-    // Tokens of the segment from this warp's next tile on; the team's warps take
-    // the chunks' pairs of tiles in turn, and all pass every chunk.
-    int left = min(s.S - s.s0 * kTileTokens, (s.s1 - s.s0) * kTileTokens) - 2 * ts * kTileTokens;
-    for (int chunks = (s.s1 - s.s0 + pl.slot_tiles - 1) / pl.slot_tiles; chunks > 0;
-         --chunks, left -= pl.slot_tiles * kTileTokens) {
-      const bool work = left > 0;
-      const unsigned char* kb = smem + slot * pl.slot_bytes + (2 * ts * pl.HG + hl) * kTile;
-      const int tile_step = pl.HG * kTile;
-      float x[2][4];
-
-      // ---- scores of two tiles ----
-      if (!__all_sync(kFull, mbar_wait(full + 8 * slot, phase))) {
-        dead = true;
-        break;
+    const int tile_step = pl.HG * kTile;
+    const unsigned char* const tiles = smem + (2 * ts * pl.HG + hl) * kTile;
+    // Adds the centres' sum to the raw sums (acc, in units of 2^-24 and, for
+    // the second dim of a pair, 2^-20) and starts it again.
+    const auto fold = [&]() {
+      #pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        #pragma unroll
+        for (int y = 0; y < NG; ++y) {
+          const float c = __shfl_sync(kFull, cw[n], 4 * y + t) * (1.f / 16777216.f);
+          #pragma unroll
+          for (int k = y * (4 / NG); k < (y + 1) * (4 / NG); ++k) {
+            a.acc[2 * k][n] += c;
+            a.acc[2 * k][2 + n] += 16.f * c;
+            a.acc[2 * k + 1][n] += c;
+            a.acc[2 * k + 1][2 + n] += 17.f * c;
+          }
+        }
+        cw[n] = 0.f;
       }
-      if (work) {
+    };
+    // One pair of tiles, `left` valid tokens in it and behind it; kTail: fewer
+    // than 32.  (Without a second tile its loads read what the slot held
+    // before; those scores are masked like the ones behind the last token.)
+    const auto pair = [&](auto tail, int left) {
+      constexpr bool kTail = decltype(tail)::value;
+      // ---- scores ----
+      if (!__all_sync(kFull, mbar_wait(full + 8 * slot, phase))) return false;
+      float x[2][4];
+      {
+        const unsigned char* kb = tiles + slot * pl.slot_bytes;
         #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          // (without a second tile this reads what the slot held before; its
-          // scores are masked like those behind the last token)
           const unsigned char* tb = kb + j * tile_step;
           const uint4 wa = lds128(tb + 64 * g + 16 * t), wb = lds128(tb + 512 + 64 * g + 16 * t);
           const uint32_t ua[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
@@ -528,8 +538,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           sb.load(tb + scale_at(8, 0, NG) + 2 * NG * g);
           ca.load(tb + k_centre_at(0, 0, NG) + 2 * NG * g);
           cb.load(tb + k_centre_at(8, 0, NG) + 2 * NG * g);
-          float sc[4];
-          mma_bf16_first(sc, ca.operand(t), cb.operand(t), sa.operand(t), sb.operand(t), qc, qs);
+          mma_bf16_first(x[j], ca.operand(t), cb.operand(t), sa.operand(t), sb.operand(t), qc, qs);
           #pragma unroll
           for (int y = 0; y < NG; ++y) {
             float d[4];
@@ -544,146 +553,164 @@ __global__ void __launch_bounds__(kThreads, 1)
                         qf[2 * k][0], qf[2 * k][1]);
               mma_f16(d, codes_n(ba), codes_n(bb), ba, bb, qf[2 * k + 1][0], qf[2 * k + 1][1]);
             }
-            sc[0] += sa[y] * d[0];
-            sc[1] += sa[y] * d[1];
-            sc[2] += sb[y] * d[2];
-            sc[3] += sb[y] * d[3];
-          }
-          #pragma unroll
-          for (int k = 0; k < 4; ++k) x[j][k] = sc[k] * fac[k & 1];
-        }
-        if (left < 2 * kTileTokens) {
-          #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            if (j * kTileTokens + g >= left) x[j][0] = x[j][1] = -INFINITY;
-            if (j * kTileTokens + g + 8 >= left) x[j][2] = x[j][3] = -INFINITY;
+            x[j][0] += sa[y] * d[0];
+            x[j][1] += sa[y] * d[1];
+            x[j][2] += sb[y] * d[2];
+            x[j][3] += sb[y] * d[3];
           }
         }
       }
       advance();
 
-      // ---- weights, and the sum over V ----
-      const unsigned char* vb = smem + slot * pl.slot_bytes + (2 * ts * pl.HG + hl) * kTile;
-      if (!__all_sync(kFull, mbar_wait(full + 8 * slot, phase))) {
-        dead = true;
-        break;
-      }
-      if (work) {
-        uint32_t pw[2][2], bw[2][2][NG];  // weights (bf16), and times the scales (fp16)
-        #pragma unroll 1
-        for (int pass = 0;; ++pass) {
-          uint32_t over = 0u;  // largest fp16 weight
-          float l[2] = {0.f, 0.f};
-          #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const unsigned char* tb = vb + j * tile_step;
-            Scales<NG> sa, sb;
-            sa.load(tb + scale_at(0, 0, NG) + 2 * NG * g);
-            sb.load(tb + scale_at(8, 0, NG) + 2 * NG * g);
-            if (left < 2 * kTileTokens) {
-              // what lies behind the last token may be anything
-              #pragma unroll
-              for (int k = 0; k < (NG + 1) / 2; ++k) {
-                if (j * kTileTokens + g >= left) sa.w[k] = 0u;
-                if (j * kTileTokens + g + 8 >= left) sb.w[k] = 0u;
-              }
-            }
-            float w[4];
-            #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              w[k] = exp2_approx(x[j][k] - a.m[k & 1]);
-              l[k & 1] += w[k];
-            }
-            pw[j][0] = pack_bf16x2(w[0], w[1]);
-            pw[j][1] = pack_bf16x2(w[2], w[3]);
-            #pragma unroll
-            for (int y = 0; y < NG; ++y) {
-              const float fa = sa[y], fb = sb[y];
-              bw[j][0][y] = pack_half2(w[0] * fa, w[1] * fa);
-              bw[j][1][y] = pack_half2(w[2] * fb, w[3] * fb);
-              over = max_half2(over, max_half2(bw[j][0][y], bw[j][1][y]));
-            }
-          }
-          // 2^15 in either half, or a weight sum that nears fp32's range
-          const bool big = (over & 0xffffu) >= 0x7800u || over >= 0x78000000u || l[0] > 1e30f ||
-                           l[1] > 1e30f;
-          if (pass == 1 || !__any_sync(kFull, big)) {
-            a.l[0] += l[0];
-            a.l[1] += l[1];
-            break;
-          }
-          float sm = 0.f;  // largest scale of a token that counts
-          #pragma unroll 1
-          for (int i = g; i < min(left, 2 * kTileTokens); i += 8) {
-            Scales<NG> sc;
-            sc.load(vb + (i / kTileTokens) * tile_step + scale_at(i % kTileTokens, 0, NG));
-            #pragma unroll
-            for (int y = 0; y < NG; ++y) sm = fmaxf(sm, sc[y]);
-          }
-          #pragma unroll
-          for (int off = 4; off < 32; off <<= 1) sm = fmaxf(sm, __shfl_xor_sync(kFull, sm, off));
-          const float room = __log2f(fminf(fmaxf(sm, 1e-18f), 1e30f)) - 9.f;
-          #pragma unroll
-          for (int n = 0; n < 2; ++n) {
-            float mx = fmaxf(fmaxf(x[0][n], x[0][2 + n]), fmaxf(x[1][n], x[1][2 + n]));
-            #pragma unroll
-            for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, off));
-            const float m = fmaxf(a.m[n], mx + room);
-            const float f = exp2_approx(a.m[n] - m);
-            a.m[n] = m;
-            a.l[n] *= f;
-            cw[n] *= f;
-            #pragma unroll
-            for (int mt = 0; mt < 8; ++mt) {
-              a.acc[mt][n] *= f;
-              a.acc[mt][2 + n] *= f;
-            }
-          }
-        }
+      // ---- weights ----
+      if (!__all_sync(kFull, mbar_wait(full + 8 * slot, phase))) return false;
+      const unsigned char* vb = tiles + slot * pl.slot_bytes;
+      uint32_t pw[2][2], bw[2][2][NG];  // weights (bf16), and times the scales (fp16)
+      #pragma unroll 1
+      for (int pass = 0;; ++pass) {
+        uint32_t over = 0u;  // largest fp16 weight
+        float l[2] = {0.f, 0.f};
         #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const int nv = left - j * kTileTokens;
-          if (j == 1 && nv <= 0) break;
           const unsigned char* tb = vb + j * tile_step;
-          const unsigned char* va = tb + 128 * t + 16 * (g ^ (2 * t));
-          const uint4 wa = lds128(va), wb = lds128(va + 512);
-          const uint32_t ua[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
-          uint32_t ca = 0u, cb = 0u;
-          if (g < NG) {
-            ca = lds32(tb + v_centre_at(0, 0, NG) + 32 * g + 4 * t);
-            cb = lds32(tb + v_centre_at(8, 0, NG) + 32 * g + 4 * t);
+          Scales<NG> sa, sb;
+          sa.load(tb + scale_at(0, 0, NG) + 2 * NG * g);
+          sb.load(tb + scale_at(8, 0, NG) + 2 * NG * g);
+          float w[4];
+          #pragma unroll
+          for (int k = 0; k < 4; ++k) w[k] = exp2_approx(x[j][k] * fac[k & 1] - a.m[k & 1]);
+          if (kTail) {
+            // what lies behind the last token may be anything
+            const bool oa = j * kTileTokens + g < left, ob = j * kTileTokens + g + 8 < left;
+            #pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              if (!oa) w[k] = 0.f;
+              if (!ob) w[2 + k] = 0.f;
+            }
+            #pragma unroll
+            for (int k = 0; k < (NG + 1) / 2; ++k) {
+              if (!oa) sa.w[k] = 0u;
+              if (!ob) sb.w[k] = 0u;
+            }
           }
-          if (nv < kTileTokens) {
-            if (2 * t >= nv) ca = 0u; else if (2 * t + 1 >= nv) ca &= 0xffffu;
-            if (2 * t + 8 >= nv) cb = 0u; else if (2 * t + 9 >= nv) cb &= 0xffffu;
-          }
-          mma_bf16(cw, ca, 0u, cb, 0u, transpose8x8(pw[j][0]), transpose8x8(pw[j][1]));
+          l[0] += w[0] + w[2];
+          l[1] += w[1] + w[3];
+          pw[j][0] = pack_bf16x2(w[0], w[1]);
+          pw[j][1] = pack_bf16x2(w[2], w[3]);
           #pragma unroll
           for (int y = 0; y < NG; ++y) {
-            const uint32_t b0 = transpose8x8(bw[j][0][y]), b1 = transpose8x8(bw[j][1][y]);
-            #pragma unroll
-            for (int k = y * (4 / NG); k < (y + 1) * (4 / NG); ++k) {
-              mma_f16(a.acc[2 * k], sub_half2(codes_n(ua[k]), 0x00080008u),
-                            sub_half2(codes_16n(ua[k]), 0x00800080u),
-                            sub_half2(codes_n(ub[k]), 0x00080008u),
-                            sub_half2(codes_16n(ub[k]), 0x00800080u), b0, b1);
-              const uint32_t ba = codes_byte(ua[k]), bb = codes_byte(ub[k]);
-              mma_f16(a.acc[2 * k + 1], sub_half2(codes_n(ba), 0x00080008u),
-                            sub_half2(ba, 0x00880088u), sub_half2(codes_n(bb), 0x00080008u),
-                            sub_half2(bb, 0x00880088u), b0, b1);
-            }
+            const float fa = sa[y], fb = sb[y];
+            bw[j][0][y] = pack_half2(w[0] * fa, w[1] * fa);
+            bw[j][1][y] = pack_half2(w[2] * fb, w[3] * fb);
+            over = max_half2(over, max_half2(bw[j][0][y], bw[j][1][y]));
+          }
+        }
+        // 2^15 in either half, or a weight sum that nears fp32's range
+        const bool big = (over & 0xffffu) >= 0x7800u || over >= 0x78000000u || l[0] + l[1] > 1e30f;
+        if (pass == 1 || !__any_sync(kFull, big)) {
+          a.l[0] += l[0];
+          a.l[1] += l[1];
+          break;
+        }
+        const int valid = kTail ? left : 2 * kTileTokens;
+        float sm = 0.f;  // largest scale of a token that counts
+        #pragma unroll 1
+        for (int i = g; i < valid; i += 8) {
+          Scales<NG> sc;
+          sc.load(vb + (i / kTileTokens) * tile_step + scale_at(i % kTileTokens, 0, NG));
+          #pragma unroll
+          for (int y = 0; y < NG; ++y) sm = fmaxf(sm, sc[y]);
+        }
+        #pragma unroll
+        for (int off = 4; off < 32; off <<= 1) sm = fmaxf(sm, __shfl_xor_sync(kFull, sm, off));
+        const float room = __log2f(fminf(fmaxf(sm, 1e-18f), 1e30f)) - 9.f;
+        #pragma unroll
+        for (int n = 0; n < 2; ++n) {
+          float mx = -INFINITY;
+          #pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            if (j * kTileTokens + g < valid) mx = fmaxf(mx, x[j][n] * fac[n]);
+            if (j * kTileTokens + g + 8 < valid) mx = fmaxf(mx, x[j][2 + n] * fac[n]);
+          }
+          #pragma unroll
+          for (int off = 4; off < 32; off <<= 1) mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, off));
+          const float m = fmaxf(a.m[n], mx + room);
+          const float f = exp2_approx(a.m[n] - m);
+          a.m[n] = m;
+          a.l[n] *= f;
+          cw[n] *= f;
+          #pragma unroll
+          for (int mt = 0; mt < 8; ++mt) {
+            a.acc[mt][n] *= f;
+            a.acc[mt][2 + n] *= f;
+          }
+        }
+      }
+
+      // ---- the sum over V ----
+      #pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const unsigned char* tb = vb + j * tile_step;
+        const unsigned char* va = tb + 128 * t + 16 * (g ^ (2 * t));
+        const uint4 wa = lds128(va), wb = lds128(va + 512);
+        const uint32_t ua[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
+        uint32_t ca = 0u, cb = 0u;
+        if (g < NG) {
+          ca = lds32(tb + v_centre_at(0, 0, NG) + 32 * g + 4 * t);
+          cb = lds32(tb + v_centre_at(8, 0, NG) + 32 * g + 4 * t);
+        }
+        if (kTail) {
+          const int nv = left - j * kTileTokens;
+          if (2 * t >= nv) ca = 0u; else if (2 * t + 1 >= nv) ca &= 0xffffu;
+          if (2 * t + 8 >= nv) cb = 0u; else if (2 * t + 9 >= nv) cb &= 0xffffu;
+        }
+        mma_bf16(cw, ca, 0u, cb, 0u, transpose8x8(pw[j][0]), transpose8x8(pw[j][1]));
+        #pragma unroll
+        for (int y = 0; y < NG; ++y) {
+          const uint32_t b0 = transpose8x8(bw[j][0][y]), b1 = transpose8x8(bw[j][1][y]);
+          const uint32_t eight = g == y ? 0xc800c800u : 0u;  // row y of -8
+          mma_f16(cw, eight, 0u, eight, 0u, b0, b1);
+          #pragma unroll
+          for (int k = y * (4 / NG); k < (y + 1) * (4 / NG); ++k) {
+            const uint32_t ba = codes_byte(ua[k]), bb = codes_byte(ub[k]);
+            mma_f16(a.acc[2 * k], codes_n(ua[k]), codes_16n(ua[k]), codes_n(ub[k]), codes_16n(ub[k]),
+                    b0, b1);
+            mma_f16(a.acc[2 * k + 1], codes_n(ba), ba, codes_n(bb), bb, b0, b1);
           }
         }
       }
       advance();
+      return true;
+    };
+
+    // Tokens of the segment from this warp's next pair on; the team's warps
+    // take the chunks' pairs in turn, and all pass every chunk.
+    int left = min(s.S - s.s0 * kTileTokens, (s.s1 - s.s0) * kTileTokens) - 2 * ts * kTileTokens;
+    int until_fold = kFold;
+    for (int chunks = (s.s1 - s.s0 + pl.slot_tiles - 1) / pl.slot_tiles; chunks > 0 && !dead;
+         --chunks, left -= pl.slot_tiles * kTileTokens) {
+      if (left >= 2 * kTileTokens) {
+        dead = !pair(std::false_type{}, left);
+      } else if (left > 0) {
+        dead = !pair(std::true_type{}, left);
+      } else {
+        for (int kv = 0; kv < 2 && !dead; ++kv) {
+          dead = !__all_sync(kFull, mbar_wait(full + 8 * slot, phase));
+          if (!dead) advance();
+        }
+      }
+      if (--until_fold == 0) {
+        fold();
+        until_fold = kFold;
+      }
     }
+    fold();
 
     // ---- segment epilogue: the warp's own sums, in full units ----
     if (dead) {
       if (lane == 0) raise_status(kStatusWaitTimeout);
       a.m[0] = a.m[1] = -INFINITY;
       a.l[0] = a.l[1] = 0.f;
-      cw[0] = cw[1] = 0.f;
       #pragma unroll
       for (int mt = 0; mt < 8; ++mt)
         a.acc[mt][0] = a.acc[mt][1] = a.acc[mt][2] = a.acc[mt][3] = 0.f;
@@ -693,17 +720,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       #pragma unroll
       for (int off = 4; off < 32; off <<= 1) a.l[n] += __shfl_xor_sync(kFull, a.l[n], off);
       #pragma unroll
-      for (int y = 0; y < NG; ++y) {
-        const float c = __shfl_sync(kFull, cw[n], 4 * y + t);
-        #pragma unroll
-        for (int k = y * (4 / NG); k < (y + 1) * (4 / NG); ++k) {
-          float(&e)[4] = a.acc[2 * k];
-          float(&o)[4] = a.acc[2 * k + 1];
-          o[2 + n] = (o[2 + n] - o[n]) * 1048576.f + c;  // a byte's 16 out' + out
-          o[n] = o[n] * 16777216.f + c;
-          e[2 + n] = e[2 + n] * 1048576.f + c;
-          e[n] = e[n] * 16777216.f + c;
-        }
+      for (int k = 0; k < 4; ++k) {
+        float(&e)[4] = a.acc[2 * k];
+        float(&o)[4] = a.acc[2 * k + 1];
+        o[2 + n] = (o[2 + n] - o[n]) * 1048576.f;  // a byte's 16 out' + out
+        o[n] *= 16777216.f;
+        e[2 + n] *= 1048576.f;
+        e[n] *= 16777216.f;
       }
     }
 
