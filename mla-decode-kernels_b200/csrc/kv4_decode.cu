@@ -21,22 +21,25 @@
 //     the end resolves.  The offset 8 joins the centres, through one product
 //     of the weights with a constant.  The raw sums grow with the context
 //     while what remains of them need not, and fp32 would lose the difference,
-//     so every kFold pairs of tiles the centres' sum is folded into them.
+//     so every kFold units the centres' sum is folded into them.
 //     The weights p_t s_ty are rounded to fp16, 2^-11.
 // The softmax reference M of a head is no running maximum but any value that
 // keeps the fp16 weights in range: it is set so that the largest p s is 2^9
 // and moves only when one passes 2^15, so the common step takes no maximum
 // and rescales nothing.
 //
-// Layout (one persistent CTA per SM, the balanced schedule of
-// gqa_balance.cuh, cut rows merged by the cut-row merge kernel):
+// Layout (one persistent CTA per SM, the balanced schedule of gqa_balance.cuh):
 //   * up to 16 consumer warps, HG x NT x TS: kv head, 8 of its q heads, and
 //     every TS-th pair of tiles; the TS warps of a head keep their own state
 //     and meet at the end of a segment;
 //   * one copy warp: a row of HG kv heads is contiguous in the cache, so one
 //     cp.async.bulk brings a tile of all of them.  A ring slot holds K or V
-//     of 2 TS tiles.  The consumers need more registers than 17 warps can
-//     share evenly, so the copy warp's group gives up most of its own.
+//     of 2 TS tiles;
+//   * three planner warps: the next segment's record and its q fragments, made
+//     while the consumers work on the current one.
+// The consumers need more registers than 20 warps can share evenly, so the
+// copy and planner warps' group gives up most of its own.  A second kernel
+// merges the rows that were cut between CTAs.
 #include <cuda_fp16.h>
 #include <math.h>
 
@@ -61,24 +64,32 @@ __device__ int g_kv4_status;
 namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
-constexpr int kMaxWarps = 16;
+constexpr int kMaxWarps = 8;                 // consumer warps
+constexpr int kUnit = 4;                     // tiles a warp works on at once
 constexpr int kMaxSlots = 16;
-constexpr int kThreads = (kMaxWarps + 4) * 32;  // and the copy warp's group
-// Registers: 640 threads at 96 are launched; 512 consumer threads at 112 and
-// 128 at 24 are 60416 of those 61440.
-constexpr int kConsumerRegs = 112, kCopyRegs = 24;
+constexpr int kPlanners = 3;
+constexpr int kThreads = (kMaxWarps + 1 + kPlanners) * 32;  // consumers, copy warp, planners
+// Registers: 384 threads at 168 are launched; 256 consumer threads at 208 and
+// 128 at 88 are those 64512.
+constexpr int kConsumerRegs = 208, kHelperRegs = 88;
 constexpr int kSmemLimit = 227 * 1024;
-constexpr int kSmemStatic = 3 * 1024;        // bound of the kernel's static shared memory
-constexpr int kPassWords = 8;                // floats per lane handed over at once at a meeting
+constexpr int kSmemStatic = 2 * 1024;        // bound of the kernel's static shared memory
+constexpr int kQWords = 20;                  // words per lane of a team's q fragments
+constexpr int kPassWords = 12;               // words per lane handed over at once at a meeting
 constexpr float kNoRef = -1e30f;             // M before the first token
-constexpr int kFold = 16;                    // pairs of tiles between two folds of the V sums
+constexpr int kFold = 8;                     // units between two folds of the V sums
 
 __device__ __forceinline__ void raise_status(int bits) { atomicOr(&g_kv4_status, bits); }
 
 // How a launch maps to warps and shared memory (no device state).
 struct Plan {
-  int G, NT, HG, NHG, TS, warps;
-  int slot_tiles, slot_bytes, nslots, smem;
+  int G;        // q heads per kv head
+  int QP, P;    // parts of P q heads each that a kv head's group is cut into (1 for G <= 64)
+  int NT;       // 8-head column tiles of a part
+  int HG, NHG;  // kv heads per row, rows per request (Hkv / HG * QP)
+  int TS, warps;
+  int slot_tiles, slot_bytes, nslots;
+  int q_at, box_at, smem;  // bytes: q fragments, meeting boxes, all dynamic shared memory
 };
 
 struct DecodeParams {
@@ -91,8 +102,7 @@ struct DecodeParams {
   float* part_m;
   float* part_l;
   float* part_acc;
-  int2* row_info;
-  int2* ends;
+  int2* row_info;  // per row {first CTA holding a part, parts}
   int B, Hq, Hkv, tiles_per_block, max_blocks, num_blocks;
   float scale_log2;
   Plan pl;
@@ -215,7 +225,7 @@ struct Seg {
 };
 
 // The CTA's share of the balanced schedule, as segments (one row, a range of
-// its tiles).  Every warp keeps its own, in shared memory.
+// its tiles).  The copy warp and each planner keep their own, in shared memory.
 struct Walk {
   long long g, g_end, row0;
   int b, hg, S, L;
@@ -270,9 +280,34 @@ __device__ __forceinline__ bool next_seg(Walk* wp, const DecodeParams& p, Seg& s
   return found;
 }
 
-__device__ __forceinline__ void group_barrier(int id, int threads) {
-  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+// Flags of a meeting, in shared memory: set and seen by single lanes, with a
+// limit on the wait.
+__device__ __forceinline__ void set_flag(uint32_t* f, uint32_t v) {
+  asm volatile("st.release.cta.shared.u32 [%0], %1;" ::"r"(smem_u32(f)), "r"(v) : "memory");
 }
+__device__ __forceinline__ bool flag_is(const uint32_t* f, uint32_t v) {
+  uint32_t x;
+  asm volatile("ld.acquire.cta.shared.u32 %0, [%1];" : "=r"(x) : "r"(smem_u32(f)) : "memory");
+  return x == v;
+}
+__device__ __forceinline__ bool wait_flag(const uint32_t* f, uint32_t v) {
+  if (flag_is(f, v)) return true;
+  const unsigned long long t0 = global_timer_ns();
+  while (true) {
+    #pragma unroll 1
+    for (int i = 0; i < 64; ++i)
+      if (flag_is(f, v)) return true;
+    if (global_timer_ns() - t0 > kWaitLimitNs) return false;
+  }
+}
+
+// What the consumers need to know of a segment.
+struct Record {
+  int valid;        // 0: no more segments
+  int b, hg, row;
+  int tiles, tokens;  // tokens: valid ones in the tiles
+  int nparts;
+};
 
 // A warp's softmax state: lane (g, t) holds heads 2 t and 2 t + 1 (n = 0, 1):
 // the reference M, the weights' sum l and dims 32 y + 4 g + 2 u + v in
@@ -281,6 +316,124 @@ struct State {
   float m[2], l[2];
   float acc[8][4];
 };
+
+// The planner warps: for each segment of the CTA its record, the row's entry
+// for the merge, and every team's q fragments (teams are dealt to the
+// planners), one segment ahead of the consumers.
+//
+// q fragments (B operand): lane (g, t) holds head g, words 4 i + t, each as
+// the dim pairs (0, 4), (1, 5), (2, 6), (3, 7) that meet the codes; then the
+// operands that meet centres and scales, 2^-24 Q and -8 2^-24 Q of the q that
+// meets the codes, and for heads 2 t and 2 t + 1 the factor that takes a sum
+// to the score in log2 units.
+template <int NG>
+__device__ __forceinline__ void plan_segments(const DecodeParams& p, Walk* walk, long long T,
+                                              long long E, int me, unsigned char* q_area,
+                                              Record* record, uint32_t filled, uint32_t read) {
+  const Plan& pl = p.pl;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  if (me == 0) {
+    // Requests without tokens occupy no tiles: CTA (b mod grid) zeroes them.
+    for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
+      if (req_len(p, b) != 0) continue;
+      for (int i = lane; i < pl.NHG; i += 32) p.row_info[b * pl.NHG + i] = make_int2(0, 0);
+      uint4* o = reinterpret_cast<uint4*>(p.out + static_cast<size_t>(b) * p.Hq * kHeadDim);
+      for (int i = lane; i < p.Hq * (kHeadDim / 8); i += 32) o[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
+  bool ok = true;  // the consumers still take records
+  for (uint32_t n = 0;; ++n) {
+    Seg s;
+    long long row_start;
+    const bool more = next_seg(walk, p, s, row_start);
+    if (ok && n > 0) ok = __all_sync(kFull, mbar_wait(read, (n - 1) & 1u));
+    if (me == 0 && lane == 0) {
+      Record r{};
+      if (more) {
+        const int tiles = tiles_of(s.S);
+        const int cfirst = static_cast<int>(range_owner(row_start, T, E));
+        r.valid = 1;
+        r.b = s.b;
+        r.hg = s.hg;
+        r.row = s.row;
+        r.tiles = s.s1 - s.s0;
+        r.tokens = min(s.S - s.s0 * kTileTokens, r.tiles * kTileTokens);
+        r.nparts = static_cast<int>(range_owner(row_start + tiles - 1, T, E)) - cfirst + 1;
+        if (s.s0 == 0) p.row_info[s.row] = make_int2(cfirst, r.nparts);
+      }
+      if (ok) *record = r;
+    }
+    if (more && ok) {
+      for (int team = me; team < pl.HG * pl.NT; team += kPlanners) {
+        const int hl = team / pl.NT, j0 = (team - hl * pl.NT) * 8;
+        const int part = s.hg % pl.QP * pl.P;
+        const bool has = j0 + g < min(pl.P, pl.G - part);
+        const uint4* qrow = reinterpret_cast<const uint4*>(
+            p.q + (static_cast<size_t>(s.b) * p.Hq + (s.hg / pl.QP * pl.HG + hl) * pl.G +
+                   (has ? part + j0 + g : 0)) * kHeadDim);
+        uint32_t* dst = reinterpret_cast<uint32_t*>(q_area + team * kQWords * 128) + lane;
+        uint32_t top = 0;  // largest |q| of the head, as bits
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint4 w = has ? __ldg(qrow + 4 * i + t) : make_uint4(0, 0, 0, 0);
+          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+          #pragma unroll
+          for (int k = 0; k < 4; ++k) top = max(top, max(u[k] & 0x7fffu, (u[k] >> 16) & 0x7fffu));
+        }
+        top = max(top, __shfl_xor_sync(kFull, top, 1));
+        top = max(top, __shfl_xor_sync(kFull, top, 2));
+        const int e = max(-100, min(100, static_cast<int>(top >> 7) - 127));
+        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);  // 2^-e
+        const float up =
+            p.scale_log2 * 16777216.f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+        dst[18 * 32] = __float_as_uint(__shfl_sync(kFull, up, 8 * t));
+        dst[19 * 32] = __float_as_uint(__shfl_sync(kFull, up, 8 * t + 4));
+        float Q[NG], R[NG];  // sums of q, and of what its roundings leave
+        #pragma unroll
+        for (int y = 0; y < NG; ++y) Q[y] = R[y] = 0.f;
+        #pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint4 w = has ? __ldg(qrow + 4 * i + t) : make_uint4(0, 0, 0, 0);
+          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+          float q[8];
+          #pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            q[2 * k] = __uint_as_float(u[k] << 16) * down;
+            q[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u) * down;
+          }
+          const float h = 0.0625f;
+          const uint32_t d = pack_half2(q[2] - q[3] * h, q[6] - q[7] * h);
+          dst[(4 * i) * 32] = pack_half2(q[0], q[4]);
+          dst[(4 * i + 1) * 32] = pack_half2(q[1] * h, q[5] * h);
+          dst[(4 * i + 2) * 32] = d;
+          dst[(4 * i + 3) * 32] = pack_half2(q[3] * h, q[7] * h);
+          const float2 df = __half22float2(*reinterpret_cast<const __half2*>(&d));
+          const float rest = q[0] + q[4] + q[1] + q[5] + q[3] + q[7];
+          float a = rest + (q[2] + q[6]);
+          float b = rest + (df.x + q[3] * h) + (df.y + q[7] * h);
+          #pragma unroll
+          for (int off = 1; off < 4; off <<= 1) {
+            a += __shfl_xor_sync(kFull, a, off);
+            b += __shfl_xor_sync(kFull, b, off);
+          }
+          Q[i * NG / 4] += a;
+          R[i * NG / 4] += b;
+        }
+        #pragma unroll
+        for (int y = 0; y < NG; ++y) {
+          Q[y] *= 1.f / 16777216.f;
+          R[y] *= -8.f / 16777216.f;
+        }
+        dst[16 * 32] = high_low<NG>(Q, t);
+        dst[17 * 32] = high_low<NG>(R, t);
+      }
+    }
+    __syncwarp();
+    if (ok && lane == 0) mbar_arrive(filled);
+    if (!more) break;
+  }
+  if (!ok && lane == 0) raise_status(kStatusWaitTimeout);
+}
 
 }  // namespace
 
@@ -292,7 +445,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ long long sh_warp[32];
   __shared__ long long sh_info[8];
   __shared__ __align__(8) unsigned long long sh_full[kMaxSlots], sh_empty[kMaxSlots];
-  __shared__ Walk sh_walk[kMaxWarps + 1];
+  __shared__ __align__(8) unsigned long long sh_seg[2];   // record filled / read
+  __shared__ Walk sh_walk[1 + kPlanners];
+  __shared__ Record sh_record;
+  __shared__ uint32_t sh_given[kMaxWarps], sh_taken[kMaxWarps];  // meetings
 
   const Plan& pl = p.pl;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -305,11 +461,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(full + 8 * i, 1);
       mbar_init(empty + 8 * i, pl.warps);
     }
+    mbar_init(smem_u32(&sh_seg[0]), kPlanners);
+    mbar_init(smem_u32(&sh_seg[1]), pl.warps);
     fence_mbar_init();
   }
+  if (threadIdx.x < kMaxWarps) sh_given[threadIdx.x] = sh_taken[threadIdx.x] = 0u;
   balanced_start(
       p.B, pl.NHG, [&](int b) -> long long { return tiles_of(req_len(p, b)); }, sh_warp, sh_info);
-  if (threadIdx.x <= kMaxWarps) {
+  if (threadIdx.x <= kPlanners) {
     Walk w;
     w.g = sh_info[0];
     w.g_end = sh_info[1];
@@ -326,28 +485,41 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp >= kMaxWarps) {
     // -------------------------------- copies --------------------------------
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCopyRegs));
-    if (warp > kMaxWarps) return;
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kHelperRegs));
+    if (warp > kMaxWarps) {
+      plan_segments<NG>(p, &sh_walk[warp - kMaxWarps], sh_info[5], sh_info[2], warp - kMaxWarps - 1,
+                        smem + pl.q_at, &sh_record, smem_u32(&sh_seg[0]), smem_u32(&sh_seg[1]));
+      return;
+    }
     const uint32_t row_bytes = static_cast<uint32_t>(pl.HG * kTile);
+    const uint64_t pol = policy_evict_first();
     int slot = 0;
     uint32_t phase = 0;
     int issued = 0;  // slots filled, counted up to nslots
     bool ok = true;
-    while (ok && next_seg(&sh_walk[kMaxWarps], p, s, row_start)) {
+    while (ok && next_seg(&sh_walk[0], p, s, row_start)) {
       const int* table = p.block_table + static_cast<size_t>(s.b) * p.max_blocks;
+      // Lane i looks up tile first + i of the row, 32 tiles at a time and one
+      // batch ahead of the copies.
+      const auto look_up = [&](int first) -> int {
+        const int tile = first + lane;
+        return tile < s.s1 ? ld_nc_s32(table + tile / p.tiles_per_block) : 0;
+      };
+      uint32_t cur = 0u;  // block * tiles per block + place in it
+      int page = look_up(s.s0);
       for (int st = s.s0; st < s.s1 && ok; st += pl.slot_tiles) {
-        const int nt = min(pl.slot_tiles, s.s1 - st);
-        size_t off = 0;
-        if (lane < nt) {
-          const int lb = (st + lane) / p.tiles_per_block, sub = st + lane - lb * p.tiles_per_block;
-          int page = ld_nc_s32(table + lb);
+        const int at = (st - s.s0) & 31;
+        if (at == 0) {
           if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_blocks)) {
             raise_status(kStatusBadPage);
             page = 0;
           }
-          off = ((static_cast<size_t>(page) * p.tiles_per_block + sub) * p.Hkv +
-                 static_cast<size_t>(s.hg) * pl.HG) * kTile;
+          cur = static_cast<uint32_t>(page) * p.tiles_per_block + (st + lane) % p.tiles_per_block;
+          page = look_up(st + 32);
         }
+        const int nt = min(pl.slot_tiles, s.s1 - st);
+        const size_t off = (static_cast<size_t>(__shfl_sync(kFull, cur, (at + lane) & 31)) * p.Hkv +
+                            s.hg / pl.QP * pl.HG) * kTile;
         for (int kv = 0; kv < 2; ++kv) {
           if (!__all_sync(kFull, mbar_wait(empty + 8 * slot, phase ^ 1))) {
             raise_status(kStatusWaitTimeout);
@@ -358,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           __syncwarp();
           if (lane < nt)
             bulk_g2s(ring + slot * pl.slot_bytes + lane * row_bytes, (kv ? p.v : p.k) + off,
-                     row_bytes, full + 8 * slot, policy_evict_first());
+                     row_bytes, full + 8 * slot, pol);
           issued = min(issued + 1, pl.nslots);
           if (++slot == pl.nslots) {
             slot = 0;
@@ -385,19 +557,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int g = lane >> 2, t = lane & 3;
   const int team = warp / pl.TS, ts = warp - team * pl.TS;  // team = (kv head, q-head tile)
   const int hl = team / pl.NT, j0 = (team - hl * pl.NT) * 8;
-  const int cnt = min(8, pl.G - j0);
-
-  // Requests without tokens occupy no tiles: CTA (b mod grid) zeroes them.
-  for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
-    if (req_len(p, b) != 0) continue;
-    if (ts == 0)
-      for (int hg = 0; hg < pl.NHG; ++hg)
-        for (int n = 0; n < cnt; ++n)
-          *reinterpret_cast<uint2*>(
-              p.out + (static_cast<size_t>(b) * p.Hq + (hg * pl.HG + hl) * pl.G + j0 + n) * kHeadDim +
-              4 * lane) = make_uint2(0, 0);
-  }
-  if (warp == 0 && lane == 0) p.ends[blockIdx.x] = make_int2(-1, 0);
 
   int slot = 0;
   uint32_t phase = 0;
@@ -409,85 +568,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       phase ^= 1;
     }
   };
-  bool dead = false;  // a wait gave up: empty states from here on (see the K1 scan)
-  bool first_seg = true;
-  while (next_seg(&sh_walk[warp], p, s, row_start)) {
-    const long long E = sh_info[2], T = sh_info[5];
-    const long long row_end = row_start + tiles_of(s.S);
-    const int cfirst = static_cast<int>(range_owner(row_start, T, E));
-    const int nparts = static_cast<int>(range_owner(row_end - 1, T, E)) - cfirst + 1;
-    if (warp == 0 && lane == 0) {
-      if (first_seg && nparts > 1 && row_start + s.s1 == row_end)
-        p.ends[blockIdx.x] = make_int2(s.row, nparts);
-      if (s.s0 == 0) p.row_info[s.row] = make_int2(cfirst, nparts);
+  bool dead = false;  // a wait gave up: this warp's rows are lost, and it ends
+  const unsigned char* const my_q = smem + pl.q_at + team * kQWords * 128 + 4 * lane;
+  uint32_t* const boxes = reinterpret_cast<uint32_t*>(smem + pl.box_at) +
+                          team * (pl.TS - 1) * kPassWords * 32 + lane;  // of the team's givers
+  uint32_t given = 0u;  // flag of this warp's last handing over
+  for (uint32_t seg = 0; !dead; ++seg) {
+    if (!__all_sync(kFull, mbar_wait(smem_u32(&sh_seg[0]), seg & 1u))) {
+      dead = true;
+      break;
     }
-    first_seg = false;
-    const int hbase = (s.hg * pl.HG + hl) * pl.G + j0;
-
-    // q fragments (B operand): lane (g, t) holds head g, words 4 i + t, each
-    // as the dim pairs (0, 4), (1, 5), (2, 6), (3, 7) that meet the codes.
-    uint32_t qf[8][2];
-    uint32_t qc, qs;  // 2^-24 Q, and -8 2^-24 Q of the q that meets the codes
-    float fac[2];     // what takes a sum to the score in log2 units
-    {
-      const bool has = g < cnt;
-      const __nv_bfloat16* qrow =
-          p.q + (static_cast<size_t>(s.b) * p.Hq + hbase + (has ? g : 0)) * kHeadDim;
-      uint4 w[4];
-      uint32_t top = 0;  // largest |q| of the head, as bits
-      #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        w[i] = has ? __ldg(reinterpret_cast<const uint4*>(qrow + 8 * (4 * i + t)))
-                   : make_uint4(0, 0, 0, 0);
-        const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-        #pragma unroll
-        for (int k = 0; k < 4; ++k) top = max(top, max(u[k] & 0x7fffu, (u[k] >> 16) & 0x7fffu));
-      }
-      top = max(top, __shfl_xor_sync(kFull, top, 1));
-      top = max(top, __shfl_xor_sync(kFull, top, 2));
-      const int e = max(-100, min(100, static_cast<int>(top >> 7) - 127));
-      const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);  // 2^-e
-      const float up =
-          p.scale_log2 * 16777216.f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-      fac[0] = __shfl_sync(kFull, up, 8 * t);
-      fac[1] = __shfl_sync(kFull, up, 8 * t + 4);
-      float Q[NG], R[NG];  // sums of q, and of what the roundings leave of it
-      #pragma unroll
-      for (int y = 0; y < NG; ++y) Q[y] = R[y] = 0.f;
-      #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const uint32_t u[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-        float q[8];
-        #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          q[2 * k] = __uint_as_float(u[k] << 16) * down;
-          q[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u) * down;
-        }
-        const float h = 0.0625f;
-        const __half d2 = __float2half_rn(q[2] - q[3] * h), d6 = __float2half_rn(q[6] - q[7] * h);
-        qf[2 * i][0] = pack_half2(q[0], q[4]);
-        qf[2 * i][1] = pack_half2(q[1] * h, q[5] * h);
-        qf[2 * i + 1][0] = pack_half2(__half2float(d2), __half2float(d6));
-        qf[2 * i + 1][1] = pack_half2(q[3] * h, q[7] * h);
-        const float rest = q[0] + q[4] + q[1] + q[5] + q[3] + q[7];
-        float a = rest + (q[2] + q[6]);
-        float b = rest + (__half2float(d2) + q[3] * h) + (__half2float(d6) + q[7] * h);
-        #pragma unroll
-        for (int off = 1; off < 4; off <<= 1) {
-          a += __shfl_xor_sync(kFull, a, off);
-          b += __shfl_xor_sync(kFull, b, off);
-        }
-        Q[i * NG / 4] += a;
-        R[i * NG / 4] += b;
-      }
-      #pragma unroll
-      for (int y = 0; y < NG; ++y) {
-        Q[y] *= 1.f / 16777216.f;
-        R[y] *= -8.f / 16777216.f;
-      }
-      qc = high_low<NG>(Q, t);
-      qs = high_low<NG>(R, t);
-    }
+    const Record r = sh_record;
+    if (!r.valid) break;
+    uint32_t qf[8][2], qc, qs;
+    float fac[2];
+    #pragma unroll
+    for (int i = 0; i < 16; ++i) qf[i / 2][i % 2] = lds32(my_q + 128 * i);
+    qc = lds32(my_q + 128 * 16);
+    qs = lds32(my_q + 128 * 17);
+    fac[0] = __uint_as_float(lds32(my_q + 128 * 18));
+    fac[1] = __uint_as_float(lds32(my_q + 128 * 19));
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&sh_seg[1]));
 
     State a;
     a.m[0] = a.m[1] = kNoRef;
@@ -498,7 +600,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     float cw[4] = {0.f, 0.f, 0.f, 0.f};
 
     const int tile_step = pl.HG * kTile;
-    const unsigned char* const tiles = smem + (2 * ts * pl.HG + hl) * kTile;
+    const unsigned char* const tiles = smem + (kUnit * ts * pl.HG + hl) * kTile;
     // Adds the centres' sum to the raw sums (acc, in units of 2^-24 and, for
     // the second dim of a pair, 2^-20) and starts it again.
     const auto fold = [&]() {
@@ -518,18 +620,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         cw[n] = 0.f;
       }
     };
-    // One pair of tiles, `left` valid tokens in it and behind it; kTail: fewer
-    // than 32.  (Without a second tile its loads read what the slot held
-    // before; those scores are masked like the ones behind the last token.)
-    const auto pair = [&](auto tail, int left) {
+    // One unit of tiles, `left` valid tokens in it and behind it; kTail: fewer
+    // than it holds.
+    const auto unit = [&](auto tail, int left) {
       constexpr bool kTail = decltype(tail)::value;
       // ---- scores ----
       if (!__all_sync(kFull, mbar_wait(full + 8 * slot, phase))) return false;
-      float x[2][4];
+      float x[kUnit][4];
       {
         const unsigned char* kb = tiles + slot * pl.slot_bytes;
         #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < kUnit; ++j) {
+          if (kTail && j * kTileTokens >= left) break;
           const unsigned char* tb = kb + j * tile_step;
           const uint4 wa = lds128(tb + 64 * g + 16 * t), wb = lds128(tb + 512 + 64 * g + 16 * t);
           const uint32_t ua[4] = {wa.x, wa.y, wa.z, wa.w}, ub[4] = {wb.x, wb.y, wb.z, wb.w};
@@ -565,13 +667,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       // ---- weights ----
       if (!__all_sync(kFull, mbar_wait(full + 8 * slot, phase))) return false;
       const unsigned char* vb = tiles + slot * pl.slot_bytes;
-      uint32_t pw[2][2], bw[2][2][NG];  // weights (bf16), and times the scales (fp16)
+      uint32_t pw[kUnit][2], bw[kUnit][2][NG];  // weights (bf16), and times the scales (fp16)
       #pragma unroll 1
       for (int pass = 0;; ++pass) {
         uint32_t over = 0u;  // largest fp16 weight
         float l[2] = {0.f, 0.f};
         #pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < kUnit; ++j) {
+          if (kTail && j * kTileTokens >= left) break;
           const unsigned char* tb = vb + j * tile_step;
           Scales<NG> sa, sb;
           sa.load(tb + scale_at(0, 0, NG) + 2 * NG * g);
@@ -612,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           a.l[1] += l[1];
           break;
         }
-        const int valid = kTail ? left : 2 * kTileTokens;
+        const int valid = kTail ? left : kUnit * kTileTokens;
         float sm = 0.f;  // largest scale of a token that counts
         #pragma unroll 1
         for (int i = g; i < valid; i += 8) {
@@ -628,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int n = 0; n < 2; ++n) {
           float mx = -INFINITY;
           #pragma unroll
-          for (int j = 0; j < 2; ++j) {
+          for (int j = 0; j < kUnit; ++j) {
             if (j * kTileTokens + g < valid) mx = fmaxf(mx, x[j][n] * fac[n]);
             if (j * kTileTokens + g + 8 < valid) mx = fmaxf(mx, x[j][2 + n] * fac[n]);
           }
@@ -649,7 +752,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
       // ---- the sum over V ----
       #pragma unroll
-      for (int j = 0; j < 2; ++j) {
+      for (int j = 0; j < kUnit; ++j) {
+        if (kTail && j * kTileTokens >= left) break;
         const unsigned char* tb = vb + j * tile_step;
         const unsigned char* va = tb + 128 * t + 16 * (g ^ (2 * t));
         const uint4 wa = lds128(va), wb = lds128(va + 512);
@@ -683,16 +787,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       return true;
     };
 
-    // Tokens of the segment from this warp's next pair on; the team's warps
-    // take the chunks' pairs in turn, and all pass every chunk.
-    int left = min(s.S - s.s0 * kTileTokens, (s.s1 - s.s0) * kTileTokens) - 2 * ts * kTileTokens;
+    // Tokens of the segment from this warp's next unit on; the team's warps
+    // take the chunks' units in turn, and all pass every chunk.
+    int left = r.tokens - kUnit * ts * kTileTokens;
     int until_fold = kFold;
-    for (int chunks = (s.s1 - s.s0 + pl.slot_tiles - 1) / pl.slot_tiles; chunks > 0 && !dead;
+    for (int chunks = (r.tiles + pl.slot_tiles - 1) / pl.slot_tiles; chunks > 0 && !dead;
          --chunks, left -= pl.slot_tiles * kTileTokens) {
-      if (left >= 2 * kTileTokens) {
-        dead = !pair(std::false_type{}, left);
+      if (left >= kUnit * kTileTokens) {
+        dead = !unit(std::false_type{}, left);
       } else if (left > 0) {
-        dead = !pair(std::true_type{}, left);
+        dead = !unit(std::true_type{}, left);
       } else {
         for (int kv = 0; kv < 2 && !dead; ++kv) {
           dead = !__all_sync(kFull, mbar_wait(full + 8 * slot, phase));
@@ -706,15 +810,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     fold();
 
+    if (dead) break;
+
     // ---- segment epilogue: the warp's own sums, in full units ----
-    if (dead) {
-      if (lane == 0) raise_status(kStatusWaitTimeout);
-      a.m[0] = a.m[1] = -INFINITY;
-      a.l[0] = a.l[1] = 0.f;
-      #pragma unroll
-      for (int mt = 0; mt < 8; ++mt)
-        a.acc[mt][0] = a.acc[mt][1] = a.acc[mt][2] = a.acc[mt][3] = 0.f;
-    }
     #pragma unroll
     for (int n = 0; n < 2; ++n) {
       #pragma unroll
@@ -730,62 +828,67 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
 
-    // ---- the team meets: halves hand over to halves, a few words at a time ----
-    const int active = min(pl.TS, (s.s1 - s.s0 + 1) / 2);  // warps of the team with tiles
-    if (active > 1) {
-      float* const scratch = reinterpret_cast<float*>(smem + pl.nslots * pl.slot_bytes) +
-                             team * (pl.TS / 2) * kPassWords * 32;
-      for (int off = pl.TS / 2; off >= 1; off >>= 1) {
-        if (off >= active) continue;  // uniform over the team
-        const bool gives = ts >= off && ts < 2 * off && ts < active;
-        const bool takes = ts < off && ts + off < active;
-        float* box = scratch + (gives ? ts - off : (takes ? ts : 0)) * kPassWords * 32 + lane;
+    // ---- the team meets: halves hand over to halves, in three passes ----
+    const int active = min(pl.TS, (r.tiles + kUnit - 1) / kUnit);  // warps of the team with tiles
+    for (int off = pl.TS / 2; off >= 1 && !dead; off >>= 1) {
+      if (ts >= off && ts < 2 * off && ts < active) {  // gives
+        uint32_t* box = boxes + (ts - 1) * kPassWords * 32;
+        #pragma unroll
+        for (int pass = 0; pass < 3; ++pass) {
+          if (!__all_sync(kFull, wait_flag(&sh_taken[warp], given))) {
+            dead = true;
+            break;
+          }
+          #pragma unroll
+          for (int k = 0; k < kPassWords; ++k) {
+            const int w = pass * kPassWords + k;
+            const float v = w < 2 ? a.m[w] : (w < 4 ? a.l[w - 2] : a.acc[(w - 4) / 4][w % 4]);
+            box[k * 32] = __float_as_uint(v);
+          }
+          __syncwarp();
+          given = 3 * seg + pass + 1;
+          if (lane == 0) set_flag(&sh_given[warp], given);
+        }
+      } else if (ts < off && ts + off < active) {  // takes
+        const uint32_t* box = boxes + (ts + off - 1) * kPassWords * 32;
         float fa[2], fo[2];
         #pragma unroll
-        for (int pass = 0; pass < 5; ++pass) {
-          if (gives) {
-            if (pass == 0) {
-              #pragma unroll
-              for (int n = 0; n < 2; ++n) {
-                box[n * 32] = a.m[n];
-                box[(2 + n) * 32] = a.l[n];
-              }
+        for (int pass = 0; pass < 3; ++pass) {
+          if (!__all_sync(kFull, wait_flag(&sh_given[warp + off], 3 * seg + pass + 1))) {
+            dead = true;
+            break;
+          }
+          #pragma unroll
+          for (int k = 0; k < kPassWords; ++k) {
+            const int w = pass * kPassWords + k;
+            const float v = __uint_as_float(box[k * 32]);
+            if (w < 2) {
+              const float m = fmaxf(a.m[w], v);
+              fa[w] = exp2_approx(a.m[w] - m);
+              fo[w] = exp2_approx(v - m);
+              a.m[w] = m;
+            } else if (w < 4) {
+              a.l[w - 2] = a.l[w - 2] * fa[w - 2] + v * fo[w - 2];
             } else {
-              #pragma unroll
-              for (int k = 0; k < kPassWords; ++k)
-                box[k * 32] = a.acc[2 * (pass - 1) + k / 4][k % 4];
+              float& o = a.acc[(w - 4) / 4][w % 4];
+              o = o * fa[w & 1] + v * fo[w & 1];
             }
           }
-          group_barrier(1 + team, 32 * pl.TS);
-          if (takes) {
-            if (pass == 0) {
-              #pragma unroll
-              for (int n = 0; n < 2; ++n) {
-                const float mo = box[n * 32], m = fmaxf(a.m[n], mo);
-                fa[n] = a.m[n] == -INFINITY ? 0.f : exp2_approx(a.m[n] - m);
-                fo[n] = mo == -INFINITY ? 0.f : exp2_approx(mo - m);
-                a.m[n] = m;
-                a.l[n] = a.l[n] * fa[n] + box[(2 + n) * 32] * fo[n];
-              }
-            } else {
-              #pragma unroll
-              for (int k = 0; k < kPassWords; ++k) {
-                float& v = a.acc[2 * (pass - 1) + k / 4][k % 4];
-                v = v * fa[k & 1] + box[k * 32] * fo[k & 1];
-              }
-            }
-          }
-          group_barrier(1 + team, 32 * pl.TS);
+          __syncwarp();
+          if (lane == 0) set_flag(&sh_taken[warp + off], 3 * seg + pass + 1);
         }
       }
     }
-    if (ts != 0) continue;
+    if (ts != 0 || dead) continue;
+    const int part = r.hg % pl.QP * pl.P;
+    const int hbase = (r.hg / pl.QP * pl.HG + hl) * pl.G + part + j0;
+    const int cnt = min(8, min(pl.P, pl.G - part) - j0);
     #pragma unroll
     for (int n = 0; n < 2; ++n) {
       const int head = 2 * t + n;
       if (head >= cnt) continue;
-      if (nparts == 1) {
-        __nv_bfloat16* o = p.out + (static_cast<size_t>(s.b) * p.Hq + hbase + head) * kHeadDim + 4 * g;
+      if (r.nparts == 1) {
+        __nv_bfloat16* o = p.out + (static_cast<size_t>(r.b) * p.Hq + hbase + head) * kHeadDim + 4 * g;
         const float inv = 1.f / a.l[n];
         #pragma unroll
         for (int y = 0; y < 4; ++y)
@@ -794,7 +897,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                          pack_bf16x2(a.acc[2 * y + 1][n] * inv, a.acc[2 * y + 1][2 + n] * inv));
       } else {
         // this CTA's slot of the row (K1's layout)
-        const size_t idx = (static_cast<size_t>(blockIdx.x) + s.row) * (pl.HG * pl.G) + hl * pl.G +
+        const size_t idx = (static_cast<size_t>(blockIdx.x) + r.row) * (pl.HG * pl.P) + hl * pl.P +
                            j0 + head;
         if (g == 0) {
           p.part_m[idx] = a.m[n];
@@ -807,6 +910,114 @@ __global__ void __launch_bounds__(kThreads, 1)
               make_float4(a.acc[2 * y][n], a.acc[2 * y][2 + n], a.acc[2 * y + 1][n],
                           a.acc[2 * y + 1][2 + n]);
       }
+    }
+  }
+  if (dead && lane == 0) raise_status(kStatusWaitTimeout);
+}
+
+struct MergeParams {
+  const int2* row_info;
+  const float* part_m;
+  const float* part_l;
+  const float* part_acc;
+  __nv_bfloat16* out;
+  int rows, QHR;  // rows, and q heads per row (HG * P)
+  int Hq, NHG, QP, HGG, G, P;  // HGG = HG * G
+};
+
+// Merge of the rows that were cut between CTAs: part k of row r is in slot
+// first + k + r.  M = max m_k, out = sum 2^(m_k - M) acc_k / sum 2^(m_k - M) l_k.
+// One warp per q head, lane = 4 dims, 16 parts in flight; kWide: the CTA's
+// warps take an eighth of one head's parts each and meet in shared memory.
+// Launched with programmatic dependent launch behind the decode.
+template <bool kWide>
+__global__ void __launch_bounds__(256) kv4_merge_kernel(const MergeParams p) {
+  constexpr int kBatch = 16;
+  __shared__ float sh_m[8], sh_l[8];
+  __shared__ float4 sh_a[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int per = kWide ? p.QHR : (p.QHR + 7) / 8;
+  const long long units = static_cast<long long>(p.rows) * per;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (long long u = blockIdx.x; u < units; u += gridDim.x) {
+    const int r = static_cast<int>(u / per);
+    const int j = static_cast<int>(u - static_cast<long long>(r) * per) * (kWide ? 1 : 8) +
+                  (kWide ? 0 : warp);
+    const int2 info = p.row_info[r];
+    const int b = r / p.NHG, hg = r - b * p.NHG, part = hg % p.QP * p.P;
+    // (kWide: uniform over the CTA)
+    if (info.y <= 1 || j >= (p.QP == 1 ? p.QHR : min(p.P, p.G - part))) continue;
+    const int k0 = kWide ? warp * info.y / 8 : 0, k1 = kWide ? (warp + 1) * info.y / 8 : info.y;
+    float M = -INFINITY, L = 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = k0; k < k1; k += kBatch) {
+      const int n = min(kBatch, k1 - k);
+      const size_t first = (static_cast<size_t>(info.x) + k + r) * p.QHR + j;
+      const size_t mine = first + static_cast<size_t>(min(lane, n - 1)) * p.QHR;
+      const float m = lane < n ? __ldcg(p.part_m + mine) : -INFINITY;
+      const float l = lane < n ? __ldcg(p.part_l + mine) : 0.f;
+      float4 x[kBatch];
+      #pragma unroll
+      for (int k = 0; k < kBatch; ++k)
+        x[k] = __ldcg(reinterpret_cast<const float4*>(
+                          p.part_acc + (first + static_cast<size_t>(min(k, n - 1)) * p.QHR) * kHeadDim) +
+                      lane);
+      float top = fmaxf(M, m);
+      #pragma unroll
+      for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, off));
+      const float f = M == -INFINITY ? 0.f : exp2f(M - top);
+      const float w = lane < n ? exp2f(m - top) : 0.f;
+      float s = l * w;
+      #pragma unroll
+      for (int off = 16; off > 0; off >>= 1) s += __shfl_xor_sync(kFull, s, off);
+      L = L * f + s;
+      a.x *= f;
+      a.y *= f;
+      a.z *= f;
+      a.w *= f;
+      #pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const float wk = __shfl_sync(kFull, w, k);
+        if (k < n) {
+          a.x += x[k].x * wk;
+          a.y += x[k].y * wk;
+          a.z += x[k].z * wk;
+          a.w += x[k].w * wk;
+        }
+      }
+      M = top;
+    }
+    if (kWide) {
+      if (lane == 0) {
+        sh_m[warp] = M;
+        sh_l[warp] = L;
+      }
+      sh_a[warp][lane] = a;
+      __syncthreads();
+      if (warp == 0) {
+        M = sh_m[0];
+        #pragma unroll
+        for (int k = 1; k < 8; ++k) M = fmaxf(M, sh_m[k]);
+        L = 0.f;
+        a = make_float4(0.f, 0.f, 0.f, 0.f);
+        #pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const float f = sh_m[k] == -INFINITY ? 0.f : exp2f(sh_m[k] - M);
+          const float4 x = sh_a[k][lane];
+          L += sh_l[k] * f;
+          a.x += x.x * f;
+          a.y += x.y * f;
+          a.z += x.z * f;
+          a.w += x.w * f;
+        }
+      }
+      __syncthreads();
+    }
+    if (!kWide || warp == 0) {
+      const float inv = 1.f / L;
+      *reinterpret_cast<uint2*>(
+          p.out + (static_cast<size_t>(b) * p.Hq + hg / p.QP * p.HGG + part + j) * kHeadDim + 4 * lane) =
+          make_uint2(pack_bf16x2(a.x * inv, a.y * inv), pack_bf16x2(a.z * inv, a.w * inv));
     }
   }
 }
@@ -887,29 +1098,34 @@ bool valid_group(int group) { return group == 32 || group == 64 || group == 128;
 int make_plan(int Hq, int Hkv, int group, Plan* p) {
   if (Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || !valid_group(group)) return -1;
   p->G = Hq / Hkv;
-  p->NT = (p->G + 7) / 8;
-  if (p->NT > kMaxWarps) return -1;
-  // kv heads per row: up to 8 warps' worth, so that at least two warps share a
-  // head's tokens (with up to 64 q heads per kv head); then as many warps per
-  // head as 16 allow.
+  if (p->G > 128) return -1;
+  const int tiles = (p->G + 7) / 8;
+  p->QP = (tiles + kMaxWarps - 1) / kMaxWarps;
+  p->NT = (tiles + p->QP - 1) / p->QP;
+  p->P = p->QP == 1 ? p->G : 8 * p->NT;
+  // kv heads per row: as many as give every warp its own head and q heads;
+  // then as many warps per head as there are left.
   p->HG = 1;
-  for (int d = 1; d <= Hkv && d * p->NT <= 8; ++d)
+  for (int d = 1; d <= Hkv && d * p->NT <= kMaxWarps; ++d)
     if (Hkv % d == 0) p->HG = d;
-  p->NHG = Hkv / p->HG;
+  p->NHG = Hkv / p->HG * p->QP;
   p->TS = 1;
   while (2 * p->TS * p->HG * p->NT <= kMaxWarps) p->TS *= 2;
   p->warps = p->HG * p->NT * p->TS;
-  p->slot_tiles = 2 * p->TS;
+  p->slot_tiles = kUnit * p->TS;
   p->slot_bytes = p->slot_tiles * p->HG * tile_bytes(group);
-  const int scratch = p->HG * p->NT * (p->TS / 2) * kPassWords * 32 * 4;
-  p->nslots = std::min(kMaxSlots, (kSmemLimit - kSmemStatic - scratch) / p->slot_bytes);
-  p->smem = p->nslots * p->slot_bytes + scratch;
+  const int q_bytes = p->HG * p->NT * kQWords * 128;
+  const int box_bytes = p->HG * p->NT * (p->TS - 1) * kPassWords * 128;
+  p->nslots = std::min(kMaxSlots, (kSmemLimit - kSmemStatic - q_bytes - box_bytes) / p->slot_bytes);
+  p->q_at = p->nslots * p->slot_bytes;
+  p->box_at = p->q_at + q_bytes;
+  p->smem = p->box_at + box_bytes;
   return 0;
 }
 
 ShapePlan shape_plan(const Plan& pl) {
   ShapePlan sp{};
-  sp.G = pl.G;
+  sp.G = pl.P;
   sp.NT = pl.NT;
   sp.HG = pl.HG;
   sp.NHG = pl.NHG;
@@ -921,6 +1137,25 @@ cudaError_t sm_count(int* sms) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   return cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev);
+}
+
+cudaError_t launch_merge(const MergeParams& p, int sms, cudaStream_t stream) {
+  // A warp per head reads up to 16 parts at once; with fewer rows than that
+  // fills, a CTA per head shares the parts of a row among its warps.
+  const bool wide = p.rows < sms / 16;
+  const long long units = wide ? static_cast<long long>(p.rows) * p.QHR
+                               : static_cast<long long>(p.rows) * ((p.QHR + 7) / 8);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min(units, 8LL * sms)));
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return wide ? cudaLaunchKernelEx(&cfg, kv4_merge_kernel<true>, p)
+              : cudaLaunchKernelEx(&cfg, kv4_merge_kernel<false>, p);
 }
 
 DeviceOnce g_smem_once;
@@ -995,7 +1230,6 @@ cudaError_t kv4_decode_launch(const gqa_bf16* q, const unsigned char* k_cache,
   p.part_l = reinterpret_cast<float*>(w + lay.l);
   p.part_acc = reinterpret_cast<float*>(w + lay.acc);
   p.row_info = reinterpret_cast<int2*>(w + lay.rowinfo);
-  p.ends = reinterpret_cast<int2*>(w + lay.ends);
   p.B = B;
   p.Hq = Hq;
   p.Hkv = Hkv;
@@ -1010,19 +1244,10 @@ cudaError_t kv4_decode_launch(const gqa_bf16* q, const unsigned char* k_cache,
   else kv4_decode_kernel<1><<<grid, threads, pl.smem, stream>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
 
-  gqa::CutMergeParams mp{};
-  mp.row_info = p.row_info;
-  mp.ends = p.ends;
-  mp.part_m = p.part_m;
-  mp.part_l = p.part_l;
-  mp.part_acc = p.part_acc;
-  mp.out = out;
-  mp.rows = B * pl.NHG;
-  mp.QHR = pl.HG * pl.G;
-  mp.grid = grid;
-  mp.out_mode = gqa::kOutBf16;
-  mp.wait_ns = gqa::kWaitLimitNs;
-  return gqa::launch_cut_merge(mp, sms, stream);
+  MergeParams mp{p.row_info,     p.part_m, p.part_l, p.part_acc, out,         B * pl.NHG,
+                 pl.HG * pl.P, Hq,       pl.NHG,   pl.QP,      pl.HG * pl.G, pl.G,
+                 pl.P};
+  return launch_merge(mp, sms, stream);
 }
 
 cudaError_t kv4_gather_launch(const unsigned char* k_cache, const unsigned char* v_cache,
