@@ -64,7 +64,7 @@ __device__ int g_kv4_status;
 namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
-constexpr int kMaxWarps = 8;                 // consumer warps
+constexpr int kMaxWarps = 8;                // consumer warps
 constexpr int kUnit = 4;                     // tiles a warp works on at once
 constexpr int kMaxSlots = 16;
 constexpr int kPlanners = 3;
@@ -88,6 +88,7 @@ struct Plan {
   int NT;       // 8-head column tiles of a part
   int HG, NHG;  // kv heads per row, rows per request (Hkv / HG * QP)
   int TS, warps;
+  int meet;     // the first step of a meeting: the power of two below TS
   int slot_tiles, slot_bytes, nslots;
   int q_at, box_at, smem;  // bytes: q fragments, meeting boxes, all dynamic shared memory
 };
@@ -139,9 +140,9 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   return r;
 }
 
-__device__ __forceinline__ uint32_t max_half2(uint32_t a, uint32_t b) {
+__device__ __forceinline__ uint32_t max_bf162(uint32_t a, uint32_t b) {
   uint32_t r;
-  asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 
@@ -309,6 +310,58 @@ struct Record {
   int nparts;
 };
 
+// The CTA's range of the balanced schedule, by one warp alone (the same cut as
+// balanced_start's, whose result in `info` is used for large batches): every
+// lane takes a run of requests.
+constexpr int kWarpStart = 512;  // largest batch of which each helper warp makes its own start
+__device__ __forceinline__ void start_walk(const DecodeParams& p, const long long* info, Walk& walk,
+                                           long long& T, long long& E) {
+  const int lane = threadIdx.x & 31, NHG = p.pl.NHG;
+  Walk w;
+  w.hg = 0;
+  if (p.B > kWarpStart) {
+    w.g = info[0];
+    w.g_end = info[1];
+    E = info[2];
+    w.b = static_cast<int>(info[3]);
+    w.row0 = info[4] * NHG;
+    T = info[5];
+  } else {
+    const int n = (p.B + 31) / 32;
+    const int lo = min(p.B, lane * n), hi = min(p.B, lo + n);
+    long long local = 0;
+    #pragma unroll 4
+    for (int b = lo; b < hi; ++b) local += tiles_of(req_len(p, b));
+    long long x = local;
+    #pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const long long y = __shfl_up_sync(kFull, x, off);
+      if (lane >= off) x += y;
+    }
+    T = __shfl_sync(kFull, x, 31) * NHG;
+    E = range_parts(T, gridDim.x);
+    w.g = range_start(blockIdx.x, T, E);
+    w.g_end = range_start(blockIdx.x + 1LL, T, E);
+    long long before = x - local;
+    const bool mine = w.g < w.g_end && w.g >= before * NHG && w.g < x * NHG;
+    int b = lo;
+    if (mine)
+      for (; b < hi; ++b) {
+        const long long L = tiles_of(req_len(p, b));
+        if (w.g < (before + L) * NHG) break;
+        before += L;
+      }
+    const unsigned who = __ballot_sync(kFull, mine);
+    const int src = who ? __ffs(who) - 1 : 0;
+    w.b = __shfl_sync(kFull, b, src);
+    w.row0 = __shfl_sync(kFull, before, src) * NHG;
+  }
+  w.S = w.g < w.g_end ? req_len(p, w.b) : 0;
+  w.L = tiles_of(w.S);
+  walk = w;  // every lane the same
+  __syncwarp();
+}
+
 // A warp's softmax state: lane (g, t) holds heads 2 t and 2 t + 1 (n = 0, 1):
 // the reference M, the weights' sum l and dims 32 y + 4 g + 2 u + v in
 // acc[2 y + u][2 v + n].
@@ -317,30 +370,89 @@ struct State {
   float acc[8][4];
 };
 
-// The planner warps: for each segment of the CTA its record, the row's entry
-// for the merge, and every team's q fragments (teams are dealt to the
-// planners), one segment ahead of the consumers.
-//
-// q fragments (B operand): lane (g, t) holds head g, words 4 i + t, each as
-// the dim pairs (0, 4), (1, 5), (2, 6), (3, 7) that meet the codes; then the
+// q fragments (B operand) of a team: lane (g, t) holds head g, words 4 i + t, each
+// as the dim pairs (0, 4), (1, 5), (2, 6), (3, 7) that meet the codes; then the
 // operands that meet centres and scales, 2^-24 Q and -8 2^-24 Q of the q that
 // meets the codes, and for heads 2 t and 2 t + 1 the factor that takes a sum
 // to the score in log2 units.
+template <int NG>
+__device__ __forceinline__ void prepare_q(const DecodeParams& p, int b, int hg, int team,
+                                          unsigned char* q_area) {
+  const Plan& pl = p.pl;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int hl = team / pl.NT, j0 = (team - hl * pl.NT) * 8;
+  const int part = hg % pl.QP * pl.P;
+  const bool has = j0 + g < min(pl.P, pl.G - part);
+  const uint4* qrow = reinterpret_cast<const uint4*>(
+      p.q + (static_cast<size_t>(b) * p.Hq + (hg / pl.QP * pl.HG + hl) * pl.G +
+             (has ? part + j0 + g : 0)) * kHeadDim);
+  uint32_t* dst = reinterpret_cast<uint32_t*>(q_area + team * kQWords * 128) + lane;
+  uint32_t top = 0;  // largest |q| of the head, as bits
+  #pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint4 w = has ? __ldg(qrow + 4 * i + t) : make_uint4(0, 0, 0, 0);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    #pragma unroll
+    for (int k = 0; k < 4; ++k) top = max(top, max(u[k] & 0x7fffu, (u[k] >> 16) & 0x7fffu));
+  }
+  top = max(top, __shfl_xor_sync(kFull, top, 1));
+  top = max(top, __shfl_xor_sync(kFull, top, 2));
+  const int e = max(-100, min(100, static_cast<int>(top >> 7) - 127));
+  const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);  // 2^-e
+  const float up =
+      p.scale_log2 * 16777216.f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+  dst[18 * 32] = __float_as_uint(__shfl_sync(kFull, up, 8 * t));
+  dst[19 * 32] = __float_as_uint(__shfl_sync(kFull, up, 8 * t + 4));
+  float Q[NG], R[NG];  // sums of q, and of what its roundings leave
+  #pragma unroll
+  for (int y = 0; y < NG; ++y) Q[y] = R[y] = 0.f;
+  #pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint4 w = has ? __ldg(qrow + 4 * i + t) : make_uint4(0, 0, 0, 0);
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+    float q[8];
+    #pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      q[2 * k] = __uint_as_float(u[k] << 16) * down;
+      q[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u) * down;
+    }
+    const float h = 0.0625f;
+    const uint32_t d = pack_half2(q[2] - q[3] * h, q[6] - q[7] * h);
+    dst[(4 * i) * 32] = pack_half2(q[0], q[4]);
+    dst[(4 * i + 1) * 32] = pack_half2(q[1] * h, q[5] * h);
+    dst[(4 * i + 2) * 32] = d;
+    dst[(4 * i + 3) * 32] = pack_half2(q[3] * h, q[7] * h);
+    const float2 df = __half22float2(*reinterpret_cast<const __half2*>(&d));
+    const float rest = q[0] + q[4] + q[1] + q[5] + q[3] + q[7];
+    float a = rest + (q[2] + q[6]);
+    float b = rest + (df.x + q[3] * h) + (df.y + q[7] * h);
+    #pragma unroll
+    for (int off = 1; off < 4; off <<= 1) {
+      a += __shfl_xor_sync(kFull, a, off);
+      b += __shfl_xor_sync(kFull, b, off);
+    }
+    Q[i * NG / 4] += a;
+    R[i * NG / 4] += b;
+  }
+  #pragma unroll
+  for (int y = 0; y < NG; ++y) {
+    Q[y] *= 1.f / 16777216.f;
+    R[y] *= -8.f / 16777216.f;
+  }
+  dst[16 * 32] = high_low<NG>(Q, t);
+  dst[17 * 32] = high_low<NG>(R, t);
+}
+
+// The planner warps: for each segment of the CTA its record, the row's entry
+// for the merge, and every team's q fragments (teams are dealt to the
+// planners), one segment ahead of the consumers, who prepare the first
+// segment's q themselves.
 template <int NG>
 __device__ __forceinline__ void plan_segments(const DecodeParams& p, Walk* walk, long long T,
                                               long long E, int me, unsigned char* q_area,
                                               Record* record, uint32_t filled, uint32_t read) {
   const Plan& pl = p.pl;
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  if (me == 0) {
-    // Requests without tokens occupy no tiles: CTA (b mod grid) zeroes them.
-    for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
-      if (req_len(p, b) != 0) continue;
-      for (int i = lane; i < pl.NHG; i += 32) p.row_info[b * pl.NHG + i] = make_int2(0, 0);
-      uint4* o = reinterpret_cast<uint4*>(p.out + static_cast<size_t>(b) * p.Hq * kHeadDim);
-      for (int i = lane; i < p.Hq * (kHeadDim / 8); i += 32) o[i] = make_uint4(0, 0, 0, 0);
-    }
-  }
+  const int lane = threadIdx.x & 31;
   bool ok = true;  // the consumers still take records
   for (uint32_t n = 0;; ++n) {
     Seg s;
@@ -363,81 +475,31 @@ __device__ __forceinline__ void plan_segments(const DecodeParams& p, Walk* walk,
       }
       if (ok) *record = r;
     }
-    if (more && ok) {
-      for (int team = me; team < pl.HG * pl.NT; team += kPlanners) {
-        const int hl = team / pl.NT, j0 = (team - hl * pl.NT) * 8;
-        const int part = s.hg % pl.QP * pl.P;
-        const bool has = j0 + g < min(pl.P, pl.G - part);
-        const uint4* qrow = reinterpret_cast<const uint4*>(
-            p.q + (static_cast<size_t>(s.b) * p.Hq + (s.hg / pl.QP * pl.HG + hl) * pl.G +
-                   (has ? part + j0 + g : 0)) * kHeadDim);
-        uint32_t* dst = reinterpret_cast<uint32_t*>(q_area + team * kQWords * 128) + lane;
-        uint32_t top = 0;  // largest |q| of the head, as bits
-        #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint4 w = has ? __ldg(qrow + 4 * i + t) : make_uint4(0, 0, 0, 0);
-          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-          #pragma unroll
-          for (int k = 0; k < 4; ++k) top = max(top, max(u[k] & 0x7fffu, (u[k] >> 16) & 0x7fffu));
-        }
-        top = max(top, __shfl_xor_sync(kFull, top, 1));
-        top = max(top, __shfl_xor_sync(kFull, top, 2));
-        const int e = max(-100, min(100, static_cast<int>(top >> 7) - 127));
-        const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);  // 2^-e
-        const float up =
-            p.scale_log2 * 16777216.f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-        dst[18 * 32] = __float_as_uint(__shfl_sync(kFull, up, 8 * t));
-        dst[19 * 32] = __float_as_uint(__shfl_sync(kFull, up, 8 * t + 4));
-        float Q[NG], R[NG];  // sums of q, and of what its roundings leave
-        #pragma unroll
-        for (int y = 0; y < NG; ++y) Q[y] = R[y] = 0.f;
-        #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint4 w = has ? __ldg(qrow + 4 * i + t) : make_uint4(0, 0, 0, 0);
-          const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-          float q[8];
-          #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            q[2 * k] = __uint_as_float(u[k] << 16) * down;
-            q[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u) * down;
-          }
-          const float h = 0.0625f;
-          const uint32_t d = pack_half2(q[2] - q[3] * h, q[6] - q[7] * h);
-          dst[(4 * i) * 32] = pack_half2(q[0], q[4]);
-          dst[(4 * i + 1) * 32] = pack_half2(q[1] * h, q[5] * h);
-          dst[(4 * i + 2) * 32] = d;
-          dst[(4 * i + 3) * 32] = pack_half2(q[3] * h, q[7] * h);
-          const float2 df = __half22float2(*reinterpret_cast<const __half2*>(&d));
-          const float rest = q[0] + q[4] + q[1] + q[5] + q[3] + q[7];
-          float a = rest + (q[2] + q[6]);
-          float b = rest + (df.x + q[3] * h) + (df.y + q[7] * h);
-          #pragma unroll
-          for (int off = 1; off < 4; off <<= 1) {
-            a += __shfl_xor_sync(kFull, a, off);
-            b += __shfl_xor_sync(kFull, b, off);
-          }
-          Q[i * NG / 4] += a;
-          R[i * NG / 4] += b;
-        }
-        #pragma unroll
-        for (int y = 0; y < NG; ++y) {
-          Q[y] *= 1.f / 16777216.f;
-          R[y] *= -8.f / 16777216.f;
-        }
-        dst[16 * 32] = high_low<NG>(Q, t);
-        dst[17 * 32] = high_low<NG>(R, t);
-      }
+    if (more && ok && n > 0) {
+      for (int team = me; team < pl.HG * pl.NT; team += kPlanners)
+        prepare_q<NG>(p, s.b, s.hg, team, q_area);
     }
     __syncwarp();
     if (ok && lane == 0) mbar_arrive(filled);
     if (!more) break;
   }
   if (!ok && lane == 0) raise_status(kStatusWaitTimeout);
+  if (me == 0) {
+    // Requests without tokens occupy no tiles: CTA (b mod grid) zeroes them.
+    for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
+      if (req_len(p, b) != 0) continue;
+      for (int i = lane; i < pl.NHG; i += 32) p.row_info[b * pl.NHG + i] = make_int2(0, 0);
+      uint4* o = reinterpret_cast<uint4*>(p.out + static_cast<size_t>(b) * p.Hq * kHeadDim);
+      for (int i = lane; i < p.Hq * (kHeadDim / 8); i += 32) o[i] = make_uint4(0, 0, 0, 0);
+    }
+  }
 }
 
 }  // namespace
 
-template <int NG>
+// kEight: HG == 8, which makes the stride between a unit's tiles a constant (3 %
+// of the time at 8 kv heads and 4 q heads each).
+template <int NG, bool kEight>
 __global__ void __launch_bounds__(kThreads, 1)
     kv4_decode_kernel(const __grid_constant__ DecodeParams p) {
   constexpr int kGroup = 128 / NG, kTile = tile_bytes(kGroup);
@@ -445,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ long long sh_warp[32];
   __shared__ long long sh_info[8];
   __shared__ __align__(8) unsigned long long sh_full[kMaxSlots], sh_empty[kMaxSlots];
-  __shared__ __align__(8) unsigned long long sh_seg[2];   // record filled / read
+  __shared__ __align__(8) unsigned long long sh_seg[3];   // record filled, read; first q ready
   __shared__ Walk sh_walk[1 + kPlanners];
   __shared__ Record sh_record;
   __shared__ uint32_t sh_given[kMaxWarps], sh_taken[kMaxWarps];  // meetings
@@ -463,22 +525,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     mbar_init(smem_u32(&sh_seg[0]), kPlanners);
     mbar_init(smem_u32(&sh_seg[1]), pl.warps);
+    mbar_init(smem_u32(&sh_seg[2]), pl.HG * pl.NT);
     fence_mbar_init();
   }
   if (threadIdx.x < kMaxWarps) sh_given[threadIdx.x] = sh_taken[threadIdx.x] = 0u;
-  balanced_start(
-      p.B, pl.NHG, [&](int b) -> long long { return tiles_of(req_len(p, b)); }, sh_warp, sh_info);
-  if (threadIdx.x <= kPlanners) {
-    Walk w;
-    w.g = sh_info[0];
-    w.g_end = sh_info[1];
-    w.b = static_cast<int>(sh_info[3]);
-    w.row0 = sh_info[4] * pl.NHG;
-    w.hg = 0;
-    w.S = w.g < w.g_end ? req_len(p, w.b) : 0;
-    w.L = tiles_of(w.S);
-    sh_walk[threadIdx.x] = w;
-  }
+  if (p.B > kWarpStart)
+    balanced_start(
+        p.B, pl.NHG, [&](int b) -> long long { return tiles_of(req_len(p, b)); }, sh_warp, sh_info);
   __syncthreads();
   Seg s;
   long long row_start;
@@ -486,9 +539,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp >= kMaxWarps) {
     // -------------------------------- copies --------------------------------
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kHelperRegs));
+    Walk& walk = sh_walk[warp - kMaxWarps];
+    long long T, E;
+    start_walk(p, sh_info, walk, T, E);
     if (warp > kMaxWarps) {
-      plan_segments<NG>(p, &sh_walk[warp - kMaxWarps], sh_info[5], sh_info[2], warp - kMaxWarps - 1,
-                        smem + pl.q_at, &sh_record, smem_u32(&sh_seg[0]), smem_u32(&sh_seg[1]));
+      plan_segments<NG>(p, &walk, T, E, warp - kMaxWarps - 1, smem + pl.q_at, &sh_record,
+                        smem_u32(&sh_seg[0]), smem_u32(&sh_seg[1]));
       return;
     }
     const uint32_t row_bytes = static_cast<uint32_t>(pl.HG * kTile);
@@ -497,29 +553,44 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t phase = 0;
     int issued = 0;  // slots filled, counted up to nslots
     bool ok = true;
-    while (ok && next_seg(&sh_walk[0], p, s, row_start)) {
-      const int* table = p.block_table + static_cast<size_t>(s.b) * p.max_blocks;
-      // Lane i looks up tile first + i of the row, 32 tiles at a time and one
-      // batch ahead of the copies.
-      const auto look_up = [&](int first) -> int {
-        const int tile = first + lane;
-        return tile < s.s1 ? ld_nc_s32(table + tile / p.tiles_per_block) : 0;
-      };
+    // Lane i looks up tile first + i of a row, a batch of tiles at a time and
+    // one batch (and one segment) ahead of the copies.
+    const int batch = 32 / pl.slot_tiles * pl.slot_tiles;
+    const bool whole = pl.HG == p.Hkv;
+    const auto look_up = [&](const Seg& q, int first) -> int {
+      const int tile = first + lane;
+      return tile < q.s1 ? ld_nc_s32(p.block_table + static_cast<size_t>(q.b) * p.max_blocks +
+                                     tile / p.tiles_per_block)
+                         : 0;
+    };
+    Seg following;
+    bool more = next_seg(&walk, p, s, row_start);
+    int page = more ? look_up(s, s.s0) : 0;
+    while (ok && more) {
       uint32_t cur = 0u;  // block * tiles per block + place in it
-      int page = look_up(s.s0);
+      int at = 0, next_page = 0;
       for (int st = s.s0; st < s.s1 && ok; st += pl.slot_tiles) {
-        const int at = (st - s.s0) & 31;
+        if (at == batch) at = 0;
         if (at == 0) {
           if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.num_blocks)) {
             raise_status(kStatusBadPage);
             page = 0;
           }
           cur = static_cast<uint32_t>(page) * p.tiles_per_block + (st + lane) % p.tiles_per_block;
-          page = look_up(st + 32);
+          page = look_up(s, st + batch);
         }
         const int nt = min(pl.slot_tiles, s.s1 - st);
-        const size_t off = (static_cast<size_t>(__shfl_sync(kFull, cur, (at + lane) & 31)) * p.Hkv +
-                            s.hg / pl.QP * pl.HG) * kTile;
+        const uint32_t tile = __shfl_sync(kFull, cur, (at + lane) & 31);
+        at += pl.slot_tiles;
+        // A row of all kv heads goes on into the next tile of its block: one
+        // copy for each run.
+        int run = lane < nt ? 1 : 0;
+        if (whole) {
+          const int sub = (st + lane) % p.tiles_per_block;
+          run = lane < nt && (lane == 0 || sub == 0) ? min(nt - lane, p.tiles_per_block - sub) : 0;
+        }
+        const size_t off =
+            (static_cast<size_t>(tile) * p.Hkv + s.hg / pl.QP * pl.HG) * kTile;
         for (int kv = 0; kv < 2; ++kv) {
           if (!__all_sync(kFull, mbar_wait(empty + 8 * slot, phase ^ 1))) {
             raise_status(kStatusWaitTimeout);
@@ -528,16 +599,22 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (lane == 0) mbar_arrive_expect_tx(full + 8 * slot, row_bytes * nt);
           __syncwarp();
-          if (lane < nt)
+          if (run > 0)
             bulk_g2s(ring + slot * pl.slot_bytes + lane * row_bytes, (kv ? p.v : p.k) + off,
-                     row_bytes, full + 8 * slot, pol);
+                     run * row_bytes, full + 8 * slot, pol);
           issued = min(issued + 1, pl.nslots);
           if (++slot == pl.nslots) {
             slot = 0;
             phase ^= 1;
           }
         }
+        if (st == s.s0) {
+          more = next_seg(&walk, p, following, row_start);
+          next_page = more ? look_up(following, following.s0) : 0;
+        }
       }
+      s = following;
+      page = next_page;
     }
     // No copy may land after the CTA has exited: wait (each with its limit)
     // for the last `issued` slots (see the K1 scan).
@@ -580,6 +657,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     const Record r = sh_record;
     if (!r.valid) break;
+    if (seg == 0) {
+      if (ts == 0) {
+        prepare_q<NG>(p, r.b, r.hg, team, smem + pl.q_at);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&sh_seg[2]));
+      }
+      if (!__all_sync(kFull, mbar_wait(smem_u32(&sh_seg[2]), 0u))) {
+        dead = true;
+        break;
+      }
+    }
     uint32_t qf[8][2], qc, qs;
     float fac[2];
     #pragma unroll
@@ -599,7 +687,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // sum_t p_t (c_ty - 8 s_ty): row y = g, heads 2 t, 2 t + 1
     float cw[4] = {0.f, 0.f, 0.f, 0.f};
 
-    const int tile_step = pl.HG * kTile;
+    const int tile_step = kEight ? 8 * kTile : pl.HG * kTile;
     const unsigned char* const tiles = smem + (kUnit * ts * pl.HG + hl) * kTile;
     // Adds the centres' sum to the raw sums (acc, in units of 2^-24 and, for
     // the second dim of a pair, 2^-20) and starts it again.
@@ -670,7 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t pw[kUnit][2], bw[kUnit][2][NG];  // weights (bf16), and times the scales (fp16)
       #pragma unroll 1
       for (int pass = 0;; ++pass) {
-        uint32_t over = 0u;  // largest fp16 weight
+        uint32_t top = 0u;  // largest scales (bf16 pairs)
         float l[2] = {0.f, 0.f};
         #pragma unroll
         for (int j = 0; j < kUnit; ++j) {
@@ -696,6 +784,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (!ob) sb.w[k] = 0u;
             }
           }
+          #pragma unroll
+          for (int k = 0; k < (NG + 1) / 2; ++k) top = max_bf162(top, max_bf162(sa.w[k], sb.w[k]));
           l[0] += w[0] + w[2];
           l[1] += w[1] + w[3];
           pw[j][0] = pack_bf16x2(w[0], w[1]);
@@ -705,11 +795,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float fa = sa[y], fb = sb[y];
             bw[j][0][y] = pack_half2(w[0] * fa, w[1] * fa);
             bw[j][1][y] = pack_half2(w[2] * fb, w[3] * fb);
-            over = max_half2(over, max_half2(bw[j][0][y], bw[j][1][y]));
           }
         }
-        // 2^15 in either half, or a weight sum that nears fp32's range
-        const bool big = (over & 0xffffu) >= 0x7800u || over >= 0x78000000u || l[0] + l[1] > 1e30f;
+        // No weight is above the lane's sum of them: neither that sum times the
+        // largest scale may pass 2^15, nor the sum near fp32's range.
+        const float most = fmaxf(l[0], l[1]);
+        const float widest = fmaxf(__uint_as_float(top << 16), __uint_as_float(top & 0xffff0000u));
+        const bool big = most * widest > 32768.f || most > 1e30f;
         if (pass == 1 || !__any_sync(kFull, big)) {
           a.l[0] += l[0];
           a.l[1] += l[1];
@@ -830,7 +922,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     // ---- the team meets: halves hand over to halves, in three passes ----
     const int active = min(pl.TS, (r.tiles + kUnit - 1) / kUnit);  // warps of the team with tiles
-    for (int off = pl.TS / 2; off >= 1 && !dead; off >>= 1) {
+    for (int off = pl.meet; off >= 1 && !dead; off >>= 1) {
       if (ts >= off && ts < 2 * off && ts < active) {  // gives
         uint32_t* box = boxes + (ts - 1) * kPassWords * 32;
         #pragma unroll
@@ -1103,15 +1195,21 @@ int make_plan(int Hq, int Hkv, int group, Plan* p) {
   p->QP = (tiles + kMaxWarps - 1) / kMaxWarps;
   p->NT = (tiles + p->QP - 1) / p->QP;
   p->P = p->QP == 1 ? p->G : 8 * p->NT;
-  // kv heads per row: as many as give every warp its own head and q heads;
-  // then as many warps per head as there are left.
-  p->HG = 1;
-  for (int d = 1; d <= Hkv && d * p->NT <= kMaxWarps; ++d)
-    if (Hkv % d == 0) p->HG = d;
+  // kv heads per row and warps per head: the most warps, and of those the most
+  // heads.  A slot's tiles have to fit the copy warp's lanes.
+  int best = 0;
+  for (int d = 1; d <= Hkv && d * p->NT <= kMaxWarps; ++d) {
+    const int ts = std::min(kMaxWarps / (d * p->NT), 32 / kUnit);
+    if (Hkv % d == 0 && d * ts >= best) {
+      best = d * ts;
+      p->HG = d;
+      p->TS = ts;
+    }
+  }
   p->NHG = Hkv / p->HG * p->QP;
-  p->TS = 1;
-  while (2 * p->TS * p->HG * p->NT <= kMaxWarps) p->TS *= 2;
   p->warps = p->HG * p->NT * p->TS;
+  p->meet = 0;
+  for (int m = 1; m < p->TS; m *= 2) p->meet = m;
   p->slot_tiles = kUnit * p->TS;
   p->slot_bytes = p->slot_tiles * p->HG * tile_bytes(group);
   const int q_bytes = p->HG * p->NT * kQWords * 128;
@@ -1160,18 +1258,24 @@ cudaError_t launch_merge(const MergeParams& p, int sms, cudaStream_t stream) {
 
 DeviceOnce g_smem_once;
 
+using DecodeKernel = void (*)(DecodeParams);
+
+DecodeKernel decode_kernel(int group, bool eight) {
+  if (group == 32) return eight ? kv4_decode_kernel<4, true> : kv4_decode_kernel<4, false>;
+  if (group == 64) return eight ? kv4_decode_kernel<2, true> : kv4_decode_kernel<2, false>;
+  return eight ? kv4_decode_kernel<1, true> : kv4_decode_kernel<1, false>;
+}
+
 cudaError_t set_smem_limits() {
   return g_smem_once.run([] {
-    const int bytes = kSmemLimit - kSmemStatic;
-    cudaError_t e = cudaFuncSetAttribute(kv4_decode_kernel<1>,
-                                         cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(kv4_decode_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               bytes);
-    if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(kv4_decode_kernel<4>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                               bytes);
-    return e;
+    for (int group : {32, 64, 128})
+      for (bool eight : {false, true}) {
+        const cudaError_t e = cudaFuncSetAttribute(decode_kernel(group, eight),
+                                                   cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                   kSmemLimit - kSmemStatic);
+        if (e != cudaSuccess) return e;
+      }
+    return cudaSuccess;
   });
 }
 
@@ -1238,10 +1342,7 @@ cudaError_t kv4_decode_launch(const gqa_bf16* q, const unsigned char* k_cache,
   p.num_blocks = num_blocks;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.pl = pl;
-  const int threads = kThreads;
-  if (group == 32) kv4_decode_kernel<4><<<grid, threads, pl.smem, stream>>>(p);
-  else if (group == 64) kv4_decode_kernel<2><<<grid, threads, pl.smem, stream>>>(p);
-  else kv4_decode_kernel<1><<<grid, threads, pl.smem, stream>>>(p);
+  decode_kernel(group, pl.HG == 8)<<<grid, kThreads, pl.smem, stream>>>(p);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
 
   MergeParams mp{p.row_info,     p.part_m, p.part_l, p.part_acc, out,         B * pl.NHG,

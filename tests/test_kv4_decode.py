@@ -111,6 +111,18 @@ def test_rows_cut_between_ctas(group, Hq, Hkv, bs, lens):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("B", [147, 512, 513, 700])
+def test_many_short_requests(B):
+    # several rows per CTA, batches on both sides of the two ways to start the
+    # schedule, a third of the requests empty
+    gen = torch.Generator().manual_seed(B)
+    lens = torch.randint(-20, 70, (B,), generator=gen).clamp(min=0).tolist()
+    c = _case(lens, 8, 2, 16, 64, seed=B)
+    _check(c, lens, _run(c, lens))
+    assert torch.equal(_run((c[0] * 0, *c[1:4]), [0] * B), torch.zeros(B, 8, 128, dtype=torch.bfloat16))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("k_scale,scale", [(8.0, SCALE), (1.0, 2.0), (0.0, SCALE), (1.0, 0.0), (1.0, -SCALE)])
 def test_peaked_and_flat_scores(k_scale, scale):
     # scores that jump by far more than the running maximum's slack, equal
