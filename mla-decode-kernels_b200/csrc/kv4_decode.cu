@@ -52,6 +52,7 @@
 #include "gqa_balance.cuh"
 #include "gqa_internal.h"
 #include "gqa_ptx.cuh"
+#include "launch_early.cuh"
 #include "kv4_decode.h"
 #include "kv4_tile.cuh"
 #include "kv_tokens.cuh"
@@ -529,6 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     fence_mbar_init();
   }
   if (threadIdx.x < kMaxWarps) sh_given[threadIdx.x] = sh_taken[threadIdx.x] = 0u;
+  wait_for_stream();
   if (p.B > kWarpStart)
     balanced_start(
         p.B, pl.NHG, [&](int b) -> long long { return tiles_of(req_len(p, b)); }, sh_warp, sh_info);
@@ -1030,7 +1032,7 @@ __global__ void __launch_bounds__(256) kv4_merge_kernel(const MergeParams p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int per = kWide ? p.QHR : (p.QHR + 7) / 8;
   const long long units = static_cast<long long>(p.rows) * per;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  wait_for_stream();
   for (long long u = blockIdx.x; u < units; u += gridDim.x) {
     const int r = static_cast<int>(u / per);
     const int j = static_cast<int>(u - static_cast<long long>(r) * per) * (kWide ? 1 : 8) +
@@ -1114,21 +1116,23 @@ __global__ void __launch_bounds__(256) kv4_merge_kernel(const MergeParams p) {
   }
 }
 
-// Read-back: half a warp per token and kv head, 8 dims per lane, K then V.
+// Read-back: a warp on one token, half a warp per kv head, 8 dims per lane;
+// nsplit warps share a token's heads where there are few tokens.
 template <int NG>
 __global__ void __launch_bounds__(256)
-    kv4_gather_kernel(Tokens tk, const unsigned char* kc, const unsigned char* vc,
-                      __nv_bfloat16* k, __nv_bfloat16* v, int Hkv) {
-  constexpr int kTile = tile_bytes(128 / NG);
+    kv4_gather_kernel(const __grid_constant__ Tokens tk, const unsigned char* kc,
+                      const unsigned char* vc, __nv_bfloat16* k, __nv_bfloat16* v, int Hkv,
+                      int nsplit) {
+  constexpr int kTile = tile_bytes(128 / NG), kBatch = 2;
   const int lane = threadIdx.x & 31, l = lane & 15;
-  const int per = (Hkv + 1) / 2;  // warps per token
   const long long w = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  if (w >= static_cast<long long>(tk.rows) * per) return;
-  const int t = static_cast<int>(w / per);
-  const int h = 2 * static_cast<int>(w - static_cast<long long>(t) * per) + (lane >> 4);
+  wait_for_stream();
+  if (w >= static_cast<long long>(tk.rows) * nsplit) return;
+  const int t = static_cast<int>(w / nsplit);
+  const int step = 2 * nsplit;
+  const int first = 2 * static_cast<int>(w - static_cast<long long>(t) * nsplit) + (lane >> 4);
   Place pl = find_place(tk, t);
-  const unsigned char* src_k = nullptr;
-  const unsigned char* src_v = nullptr;
+  size_t off = 0;  // of the token's tile of head 0
   int ti = 0;
   if (pl.live) {
     if (pl.pos >= static_cast<long long>(tk.max_blocks) * tk.block_size) {
@@ -1142,42 +1146,54 @@ __global__ void __launch_bounds__(256)
         page = 0;
       }
       ti = slot % kTileTokens;
-      const size_t off = ((static_cast<size_t>(page) * (tk.block_size / kTileTokens) +
-                           slot / kTileTokens) * Hkv + h) * kTile;
-      src_k = kc + off;
-      src_v = vc + off;
+      off = (static_cast<size_t>(page) * (tk.block_size / kTileTokens) + slot / kTileTokens) * Hkv *
+            kTile;
     }
   }
-  if (h >= Hkv) return;
-  uint4 ok = make_uint4(0, 0, 0, 0), ov = ok;
-  if (pl.live) {
-    const int y = 8 * l * NG / 128;
-    const auto half = [](const unsigned char* a) {
-      return __uint_as_float(
-          static_cast<unsigned>(__ldg(reinterpret_cast<const unsigned short*>(a))) << 16);
-    };
-    const unsigned ck = __ldg(reinterpret_cast<const unsigned*>(src_k + k_word(ti, l)));
-    const unsigned cv =
-        __ldg(reinterpret_cast<const unsigned short*>(src_v + v_half(ti, 2 * l))) |
-        static_cast<unsigned>(
-            __ldg(reinterpret_cast<const unsigned short*>(src_v + v_half(ti, 2 * l + 1)))) << 16;
-    const float sk = half(src_k + scale_at(ti, y, NG)), zk = half(src_k + k_centre_at(ti, y, NG));
-    const float sv = half(src_v + scale_at(ti, y, NG)), zv = half(src_v + v_centre_at(ti, y, NG));
-    const auto value = [](unsigned w, int i, float sc, float c) {
-      return __fadd_rn(__fmul_rn(static_cast<float>(static_cast<int>((w >> (4 * i)) & 15u) - 8), sc), c);
-    };
-    unsigned a[4], b[4];
+  const int y = 8 * l * NG / 128;
+  const int ck = k_word(ti, l), cv = v_half(ti, 2 * l), cv2 = v_half(ti, 2 * l + 1);
+  const int sc = scale_at(ti, y, NG), zk = k_centre_at(ti, y, NG), zv = v_centre_at(ti, y, NG);
+  const auto ld16 = [](const unsigned char* a) -> unsigned {
+    return __ldg(reinterpret_cast<const unsigned short*>(a));
+  };
+  // s (n - 8) + c: n as the last bits of 2^23 + n; the product is exact.
+  const auto value = [](unsigned w, int i, unsigned s, unsigned c) {
+    const float n = __uint_as_float(((w >> (4 * i)) & 15u) | 0x4b000000u) - 8388616.f;
+    return fmaf(n, __uint_as_float(s << 16), __uint_as_float(c << 16));
+  };
+  const auto pack = [&](unsigned w, unsigned s, unsigned c) {
+    unsigned r[4];
     #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      a[i] = pack_bf16x2(value(ck, 2 * i, sk, zk), value(ck, 2 * i + 1, sk, zk));
-      b[i] = pack_bf16x2(value(cv, 2 * i, sv, zv), value(cv, 2 * i + 1, sv, zv));
+    for (int i = 0; i < 4; ++i)
+      r[i] = pack_bf16x2(value(w, 2 * i, s, c), value(w, 2 * i + 1, s, c));
+    return make_uint4(r[0], r[1], r[2], r[3]);
+  };
+  const size_t out = static_cast<size_t>(t) * Hkv * 128 + 8 * l;
+  for (int h0 = first; h0 < Hkv; h0 += kBatch * step) {
+    unsigned wk[kBatch], wv[kBatch], sk[kBatch], sv[kBatch], ok[kBatch], ov[kBatch];
+    #pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int h = h0 + i * step;
+      wk[i] = wv[i] = sk[i] = sv[i] = ok[i] = ov[i] = 0u;
+      if (pl.live && h < Hkv) {
+        const unsigned char* a = kc + off + static_cast<size_t>(h) * kTile;
+        const unsigned char* b = vc + off + static_cast<size_t>(h) * kTile;
+        wk[i] = __ldg(reinterpret_cast<const unsigned*>(a + ck));
+        wv[i] = ld16(b + cv) | ld16(b + cv2) << 16;
+        sk[i] = ld16(a + sc);
+        ok[i] = ld16(a + zk);
+        sv[i] = ld16(b + sc);
+        ov[i] = ld16(b + zv);
+      }
     }
-    ok = make_uint4(a[0], a[1], a[2], a[3]);
-    ov = make_uint4(b[0], b[1], b[2], b[3]);
+    #pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int h = h0 + i * step;
+      if (h >= Hkv) break;
+      *reinterpret_cast<uint4*>(k + out + static_cast<size_t>(h) * 128) = pack(wk[i], sk[i], ok[i]);
+      *reinterpret_cast<uint4*>(v + out + static_cast<size_t>(h) * 128) = pack(wv[i], sv[i], ov[i]);
+    }
   }
-  const size_t at = (static_cast<size_t>(t) * Hkv + h) * 128 + 8 * l;
-  *reinterpret_cast<uint4*>(k + at) = ok;
-  *reinterpret_cast<uint4*>(v + at) = ov;
 }
 
 namespace {
@@ -1243,17 +1259,8 @@ cudaError_t launch_merge(const MergeParams& p, int sms, cudaStream_t stream) {
   const bool wide = p.rows < sms / 16;
   const long long units = wide ? static_cast<long long>(p.rows) * p.QHR
                                : static_cast<long long>(p.rows) * ((p.QHR + 7) / 8);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min(units, 8LL * sms)));
-  cfg.blockDim = dim3(256);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return wide ? cudaLaunchKernelEx(&cfg, kv4_merge_kernel<true>, p)
-              : cudaLaunchKernelEx(&cfg, kv4_merge_kernel<false>, p);
+  return launch_early(wide ? kv4_merge_kernel<true> : kv4_merge_kernel<false>,
+                      static_cast<int>(std::min(units, 8LL * sms)), 256, 0, stream, p);
 }
 
 DeviceOnce g_smem_once;
@@ -1342,8 +1349,8 @@ cudaError_t kv4_decode_launch(const gqa_bf16* q, const unsigned char* k_cache,
   p.num_blocks = num_blocks;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.pl = pl;
-  decode_kernel(group, pl.HG == 8)<<<grid, kThreads, pl.smem, stream>>>(p);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  e = gqa::launch_early(decode_kernel(group, pl.HG == 8), grid, kThreads, pl.smem, stream, p);
+  if (e != cudaSuccess) return e;
 
   MergeParams mp{p.row_info,     p.part_m, p.part_l, p.part_acc, out,         B * pl.NHG,
                  pl.HG * pl.P, Hq,       pl.NHG,   pl.QP,      pl.HG * pl.G, pl.G,
@@ -1368,13 +1375,15 @@ cudaError_t kv4_gather_launch(const unsigned char* k_cache, const unsigned char*
     return cudaErrorMisalignedAddress;
   const gqa::Tokens tk{block_table, seq_lens, cu_seqlens, nullptr,   rows,
                        B,           max_blocks, num_blocks, block_size};
-  const long long grid = (static_cast<long long>(rows) * ((Hkv + 1) / 2) + 7) / 8;
+  // One wave of warps (eight CTAs of eight on every SM) or a warp per token.
+  const int nsplit = std::max(1, std::min(148 * 64 / rows, (Hkv + 1) / 2));
+  const long long grid = (static_cast<long long>(rows) * nsplit + 7) / 8;
   if (grid > INT_MAX) return cudaErrorInvalidValue;
-  const int g = static_cast<int>(grid);
-  if (group == 32) kv4_gather_kernel<4><<<g, 256, 0, stream>>>(tk, k_cache, v_cache, k, v, Hkv);
-  else if (group == 64) kv4_gather_kernel<2><<<g, 256, 0, stream>>>(tk, k_cache, v_cache, k, v, Hkv);
-  else kv4_gather_kernel<1><<<g, 256, 0, stream>>>(tk, k_cache, v_cache, k, v, Hkv);
-  return cudaGetLastError();
+  const auto kernel = group == 32   ? kv4_gather_kernel<4>
+                      : group == 64 ? kv4_gather_kernel<2>
+                                    : kv4_gather_kernel<1>;
+  return gqa::launch_early(kernel, static_cast<int>(grid), 256, 0, stream, tk, k_cache, v_cache, k, v,
+                           Hkv, nsplit);
 }
 
 int kv4_decode_get_status(int reset) {

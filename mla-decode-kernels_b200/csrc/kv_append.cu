@@ -8,12 +8,12 @@
 //
 // The pass is bound by memory: every byte of q, k and v is read once and
 // written once and nothing is kept in between.  A head row is 256 bytes, so
-// half a warp holds it, 8 dims (16 bytes) per lane: the norm's sum is four
-// shuffles, a pair of the half layout is one shuffle apart (rotary_dim / 16
-// lanes) and an interleaved pair sits in one lane.  A warp works on one token
-// and keeps its row of the cosine / sine table in registers over all the
-// heads it takes; small calls give every warp fewer heads instead, down to
-// one row per half warp, so that one token's heads run side by side.
+// half a warp holds it, 8 dims per lane: in the half layout the 4 dims of a
+// rotation's first half and the 4 of its second, so that a pair never leaves
+// its lane; the norm's sum is four shuffles.  A warp works on one token and
+// keeps its angles, multiplied by the norm's weights, in registers over all
+// the heads it takes; small calls give every warp fewer heads instead, down
+// to one row per half warp, so that one token's heads run side by side.
 #include <cuda_bf16.h>
 #include <math.h>
 
@@ -21,6 +21,7 @@
 #include <cstdint>
 
 #include "gqa_ptx.cuh"
+#include "launch_early.cuh"
 #include "kv4_tile.cuh"
 #include "kv_append.h"
 #include "kv_tokens.cuh"
@@ -32,7 +33,8 @@ __device__ int g_append_status;
 
 constexpr unsigned kFull = 0xffffffffu;
 constexpr int kThreads = 256;
-constexpr int kBatch = 4;  // head rows a half warp loads before it works on them
+constexpr int kBatch = 4;     // head rows a half warp loads before it works on them
+constexpr int kMlaBatch = 8;  // and a quarter warp, of 128 bytes each
 
 enum Rope : int { kNoRope = 0, kHalves = 1, kPairs = 2 };
 
@@ -66,8 +68,16 @@ __device__ __forceinline__ void raise_status(int bits) { atomicOr(&g_append_stat
 
 __device__ __forceinline__ uint4 ld_stream(const void* p) {
   uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
                : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ uint2 ld_stream8(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.L1::no_allocate.v2.u32 {%0, %1}, [%2];"
+               : "=r"(v.x), "=r"(v.y)
                : "l"(p));
   return v;
 }
@@ -86,16 +96,16 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
                     pack_bf16x2(x[6], x[7]));
 }
 
-// Weights of dims d .. d + 7.
-__device__ __forceinline__ void load_weight(const Norm& n, int d, float (&w)[8]) {
+// Weights of dims d .. d + 3.
+__device__ __forceinline__ void load_weight4(const Norm& n, int d, float* w) {
   if (n.fp32) {
-    const float4* f = reinterpret_cast<const float4*>(static_cast<const float*>(n.weight) + d);
-    const float4 a = __ldg(f), b = __ldg(f + 1);
+    const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(n.weight) + d));
     w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
-    w[4] = b.x; w[5] = b.y; w[6] = b.z; w[7] = b.w;
   } else {
-    unpack8(__ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(n.weight) + d)),
-            w);
+    const uint2 a =
+        __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(n.weight) + d));
+    w[0] = __uint_as_float(a.x << 16); w[1] = __uint_as_float(a.x & 0xffff0000u);
+    w[2] = __uint_as_float(a.y << 16); w[3] = __uint_as_float(a.y & 0xffff0000u);
   }
 }
 
@@ -154,81 +164,281 @@ __device__ __forceinline__ void rotate(float (&x)[8], const Angles& a, int rot, 
   }
 }
 
-__device__ __forceinline__ float max_nan(float a, float b) {
+// Minimum and maximum that keep a NaN.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
   float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 
-__device__ __forceinline__ float min_nan(float a, float b) {
+__device__ __forceinline__ float min_nan(float a, float b, float c) {
   float r;
-  asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
+}
+
+// a / b from an approximate 1 / b, corrected by the remainder (Markstein's
+// method): a quotient that fp32 holds exactly, such as one half way between
+// two codes, comes out exactly.
+__device__ __forceinline__ float quotient(float a, float b, float inv) {
+  const float q = __fmul_rn(a, inv);
+  return __fmaf_rn(__fmaf_rn(-q, b, a), inv, q);
 }
 
 // The 4-bit codes of x (8 dims; the group's other dims in the neighbouring
 // lanes), and the group's scale and centre.  Every lane must call it.
 __device__ __forceinline__ unsigned quantise(const float (&x)[8], int group, unsigned short& s16,
                                              unsigned short& c16) {
-  float lo = x[0], hi = x[0];
-  #pragma unroll
-  for (int i = 1; i < 8; ++i) {
-    lo = min_nan(lo, x[i]);
-    hi = max_nan(hi, x[i]);
-  }
-  for (int off = 1; off < group / 8; off <<= 1) {
-    lo = min_nan(lo, __shfl_xor_sync(kFull, lo, off));
-    hi = max_nan(hi, __shfl_xor_sync(kFull, hi, off));
+  float lo = min_nan(min_nan(x[0], x[1], x[2]), min_nan(x[3], x[4], x[5]), x[6]);
+  float hi = max_nan(max_nan(x[0], x[1], x[2]), max_nan(x[3], x[4], x[5]), x[6]);
+  const float o = __shfl_xor_sync(kFull, min_nan(lo, x[7], x[7]), 1);
+  const float u = __shfl_xor_sync(kFull, max_nan(hi, x[7], x[7]), 1);
+  lo = min_nan(lo, x[7], o);
+  hi = max_nan(hi, x[7], u);
+  for (int off = 2; off < group / 8; off <<= 1) {
+    const float a = __shfl_xor_sync(kFull, lo, off), b = __shfl_xor_sync(kFull, hi, off);
+    lo = min_nan(lo, a, a);
+    hi = max_nan(hi, b, b);
   }
   // Rounded up to bf16, so that 15 steps span the group (a NaN stays one).
-  const float want = __fdiv_rn(__fsub_rn(hi, lo), 15.f);
+  const float want = quotient(__fsub_rn(hi, lo), 15.f, 1.f / 15.f);
   const float s = want != want ? want
                                : __uint_as_float((__float_as_uint(want) + 0xffffu) & 0xffff0000u);
   const __nv_bfloat16 cb = __float2bfloat16(__fadd_rn(lo, __fmul_rn(8.f, s)));
   const float c = __bfloat162float(cb);
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  if (s == 0.f) inv = 0.f;  // the group is one value up to the rounding of c: n = 8
   unsigned w = 0;
   #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    // s = 0: 0 / 0 or +-y / 0; the NaN converts to 0, and the group is one
-    // value up to the rounding of c
-    int n = s == 0.f ? 0 : __float2int_rn(__fdiv_rn(__fsub_rn(x[i], c), s));
-    n = max(-8, min(7, n)) + 8;
-    w |= static_cast<unsigned>(n) << (4 * i);
+  for (int i = 6; i >= 0; i -= 2) {
+    const int n0 = __float2int_rn(quotient(__fsub_rn(x[i], c), s, inv));
+    const int n1 = __float2int_rn(quotient(__fsub_rn(x[i + 1], c), s, inv));
+    // clamped to [-8, 7] and put below what is there
+    asm("cvt.pack.sat.s4.s32.b32 %0, %1, %2, %0;" : "+r"(w) : "r"(n1), "r"(n0));
   }
+  w ^= 0x88888888u;  // + 8
   s16 = static_cast<unsigned short>(__float_as_uint(s) >> 16);
   if (s != s) s16 = 0x7fc0;
   c16 = __bfloat16_as_ushort(cb);
   return w;
 }
 
-template <int MODE, bool KV4>
-__global__ void __launch_bounds__(kThreads)
-    kv_append_gqa_kernel(const __grid_constant__ GqaParams p, int group) {
-  const int lane = threadIdx.x & 31, half = lane >> 4, l = lane & 15;
-  const long long w = static_cast<long long>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
-  if (w >= static_cast<long long>(p.tk.rows) * p.nsplit) return;
-  const int t = static_cast<int>(w / p.nsplit);
-  const int split = static_cast<int>(w - static_cast<long long>(t) * p.nsplit);
-  const int nrows = p.Hq + 2 * p.Hkv;
-  const int step = 2 * p.nsplit;
+// How the 16 lanes of a half warp hold a head's 128 dims, as four pairs
+// (a_i, b_i) each that rotate together: in the half layout dims 4 l + i and
+// rot / 2 + 4 l + i for the lanes l < rot / 8 and eight consecutive dims that
+// do not rotate for the others; else dims 8 l + 2 i and 8 l + 2 i + 1.
+template <int MODE>
+struct Lay {
+  int at0, at1;  // first dims of the lane's two runs of four
+  bool on;       // the lane's pairs rotate
 
-  // One batch of this half warp's head rows: q heads, then k, then v.
-  auto src = [&](int r) {
-    const __nv_bfloat16* b;
-    if (r < p.Hq) b = p.q.data + t * p.q.tok + r * p.q.head;
-    else if (r < p.Hq + p.Hkv) b = p.k.data + t * p.k.tok + (r - p.Hq) * p.k.head;
-    else b = p.v.data + t * p.v.tok + (r - p.Hq - p.Hkv) * p.v.head;
-    return b + 8 * l;
-  };
+  __device__ __forceinline__ Lay(int rot, int l) {
+    on = MODE != kNoRope && l < rot / 8;
+    at0 = 8 * l;
+    at1 = at0 + 4;
+    if (MODE == kHalves && on) {
+      at0 = 4 * l;
+      at1 = rot / 2 + 4 * l;
+    }
+  }
+  __device__ __forceinline__ uint4 load(const __nv_bfloat16* row) const {
+    if (MODE != kHalves) return ld_stream(row + at0);
+    const uint2 x = ld_stream8(row + at0), y = ld_stream8(row + at1);
+    return make_uint4(x.x, x.y, y.x, y.y);
+  }
+  __device__ __forceinline__ void store(__nv_bfloat16* row, const uint4& v) const {
+    if (MODE != kHalves) {
+      *reinterpret_cast<uint4*>(row + at0) = v;
+    } else {
+      *reinterpret_cast<uint2*>(row + at0) = make_uint2(v.x, v.y);
+      *reinterpret_cast<uint2*>(row + at1) = make_uint2(v.z, v.w);
+    }
+  }
+  // Place of element i of pair member m (0: a, 1: b) in the eight loaded values.
+  static __device__ __forceinline__ constexpr int at(int i, int m) {
+    return MODE == kHalves ? 4 * m + i : 2 * i + m;
+  }
+};
+
+// y = f (a C - b S), f (b C' + a S'): cosines and sines times the weights, f
+// the norm's factor.
+struct Turn {
+  float ca[4], sb[4], cb[4], sa[4];
+};
+
+template <int MODE>
+__device__ __forceinline__ void make_turn(const Norm& n, const float* angles, int rot, int l,
+                                          const Lay<MODE>& lay, Turn& u) {
+  float w[8];
+  #pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = 1.f;
+  if (n.weight) load_weight4(n, lay.at0, w), load_weight4(n, lay.at1, w + 4);
+  float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (lay.on) {
+    c = __ldg(reinterpret_cast<const float4*>(angles + 4 * l));
+    s = __ldg(reinterpret_cast<const float4*>(angles + rot / 2 + 4 * l));
+  }
+  const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+  #pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float wa = w[Lay<MODE>::at(i, 0)], wb = w[Lay<MODE>::at(i, 1)];
+    u.ca[i] = wa * cc[i];
+    u.sb[i] = wb * ss[i];
+    u.cb[i] = wb * cc[i];
+    u.sa[i] = wa * ss[i];
+  }
+}
+
+// Norm and rotation of the bf16 head rows first, first + step, ... < count of
+// one token; every lane of the warp takes part, half 1 one row behind half 0
+// (rows may differ between the halves, `iters` may not).  At dst rows are
+// dst_stride apart.
+template <int MODE>
+__device__ __forceinline__ void turn_rows(const Lay<MODE>& lay, const __nv_bfloat16* src, long long stride, int first,
+                                          int step, int iters, int count, const Norm& n,
+                                          const float* angles, int rot, __nv_bfloat16* dst,
+                                          long long dst_stride) {
+  const int l = threadIdx.x & 15;
   uint4 raw[kBatch];
-  auto load = [&](int base) {
+  const auto load = [&](int i0) {
     #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const int r = base + i * step + half;
-      raw[i] = r < nrows ? ld_stream(src(r)) : make_uint4(0, 0, 0, 0);
+      const int r = first + (i0 + i) * step;
+      raw[i] = i0 + i < iters && r < count ? lay.load(src + r * stride) : make_uint4(0, 0, 0, 0);
     }
   };
-  load(2 * split);  // in flight while the token's place is looked up
+  if (iters == 0) return;
+  load(0);
+  Turn u;
+  make_turn<MODE>(n, angles, rot, l, lay, u);
+  const bool partial = MODE != kNoRope && rot < 128;
+  for (int i0 = 0; i0 < iters; i0 += kBatch) {
+    if (i0) load(i0);
+    #pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (i0 + i >= iters) break;
+      const int r = first + (i0 + i) * step;
+      float x[8];
+      unpack8(raw[i], x);
+      if (n.weight) {
+        float ss = 0.f;
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) ss = fmaf(x[j], x[j], ss);
+        #pragma unroll
+        for (int off = 1; off < 16; off <<= 1) ss += __shfl_xor_sync(kFull, ss, off);
+        const float f = rsqrtf(fmaf(ss, 1.f / 128.f, n.eps));
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] *= f;
+      }
+      float y[8];
+      #pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float a = x[Lay<MODE>::at(j, 0)], b = x[Lay<MODE>::at(j, 1)];
+        if (MODE == kNoRope) {
+          y[Lay<MODE>::at(j, 0)] = a * u.ca[j];
+          y[Lay<MODE>::at(j, 1)] = b * u.cb[j];
+        } else {
+          // (an infinity that does not rotate must not meet a sine of 0)
+          const float a1 = partial && !lay.on ? 0.f : a, b1 = partial && !lay.on ? 0.f : b;
+          y[Lay<MODE>::at(j, 0)] = fmaf(a, u.ca[j], -(b1 * u.sb[j]));
+          y[Lay<MODE>::at(j, 1)] = fmaf(b, u.cb[j], a1 * u.sa[j]);
+        }
+      }
+      if (r < count) lay.store(dst + r * dst_stride, pack8(y));
+    }
+  }
+}
+
+// K (normed, rotated) or V rows of one token into its tiles of the 4-bit
+// cache; 8 consecutive dims per lane.  K's fp32 operations are rounded one by
+// one, in the formula's order, so that equal inputs give equal codes wherever
+// they are computed.
+template <int MODE, bool kValue>
+__device__ __forceinline__ void quantise_rows(const __nv_bfloat16* src, long long stride,
+                                              int first, int step, int iters,
+                                              int count, const Norm& n,
+                                              const float* angles, int rot, unsigned char* tile,
+                                              int ti, int group) {
+  if (iters == 0) return;
+  const int l = threadIdx.x & 15, ng = 128 / group, y = 8 * l / group;
+  Angles ang;
+  if (!kValue) load_angles<MODE>(angles, rot, l, ang);
+  float wt[8];
+  if (!kValue && n.weight) {
+    load_weight4(n, 8 * l, wt);
+    load_weight4(n, 8 * l + 4, wt + 4);
+  }
+  for (int i0 = 0; i0 < iters; i0 += kBatch) {
+    uint4 raw[kBatch];
+    #pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int r = first + (i0 + i) * step;
+      raw[i] = i0 + i < iters && r < count ? ld_stream(src + r * stride + 8 * l)
+                                           : make_uint4(0, 0, 0, 0);
+    }
+    #pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (i0 + i >= iters) break;
+      const int r = first + (i0 + i) * step;
+      float x[8];
+      unpack8(raw[i], x);
+      if (!kValue) {
+        if (n.weight) {
+          float ss = 0.f;
+          #pragma unroll
+          for (int j = 0; j < 8; ++j) ss += x[j] * x[j];
+          #pragma unroll
+          for (int off = 1; off < 16; off <<= 1) ss += __shfl_xor_sync(kFull, ss, off);
+          const float f = rsqrtf(ss * (1.f / 128.f) + n.eps);
+          #pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] = x[j] * f * wt[j];
+        }
+        rotate<MODE>(x, ang, rot, l, true);
+      }
+      unsigned short s16, c16;
+      const unsigned codes = quantise(x, group, s16, c16);
+      if (r >= count || !tile) continue;
+      unsigned char* at = tile + static_cast<size_t>(r) * kv4::tile_bytes(group);
+      if (kValue) {
+        *reinterpret_cast<unsigned short*>(at + kv4::v_half(ti, 2 * l)) =
+            static_cast<unsigned short>(codes);
+        *reinterpret_cast<unsigned short*>(at + kv4::v_half(ti, 2 * l + 1)) =
+            static_cast<unsigned short>(codes >> 16);
+      } else {
+        *reinterpret_cast<unsigned*>(at + kv4::k_word(ti, l)) = codes;
+      }
+      if (8 * l % group == 0) {
+        *reinterpret_cast<unsigned short*>(at + kv4::scale_at(ti, y, ng)) = s16;
+        *reinterpret_cast<unsigned short*>(
+            at + (kValue ? kv4::v_centre_at(ti, y, ng) : kv4::k_centre_at(ti, y, ng))) = c16;
+      }
+    }
+  }
+}
+
+template <int MODE, bool KV4>
+__global__ void __launch_bounds__(kThreads, 4)
+    kv_append_gqa_kernel(const __grid_constant__ GqaParams p, int group) {
+  const int lane = threadIdx.x & 31, l = lane & 15;
+  const long long w = static_cast<long long>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  wait_for_stream();
+  if (w >= static_cast<long long>(p.tk.rows) * p.nsplit) return;
+  const int t = static_cast<int>(w / p.nsplit);
+  // This half warp takes every step-th of the token's rows: q heads, k, v.
+  const int step = 2 * p.nsplit;
+  const int mine = 2 * static_cast<int>(w - static_cast<long long>(t) * p.nsplit) + (lane >> 4);
+  const auto first = [&](int before) { return ((mine - before) % step + step) % step; };
+  // Steps that bring every row's turn; none where neither half has a row.
+  const auto iters = [&](int from, int count) {
+    return __any_sync(kFull, from < count) ? (count + step - 1) / step : 0;
+  };
+
+  const int k_first = first(p.Hq), v_first = first(p.Hq + p.Hkv);
+  const __nv_bfloat16* const q = p.q.data + t * p.q.tok;
+  const __nv_bfloat16* const k = p.k.data + t * p.k.tok;
+  const __nv_bfloat16* const v = p.v.data + t * p.v.tok;
+  const Lay<MODE> lay(p.rot, l);
 
   Place pl = find_place(p.tk, t);
   int bad = 0;
@@ -247,79 +457,41 @@ __global__ void __launch_bounds__(kThreads)
       page = -1;
     }
   }
-  if (bad && split == 0 && lane == 0) raise_status(bad);
+  if (bad && mine < 2 && lane == 0) raise_status(bad);
   if (!pl.live) {
     if (p.zero_skipped)
-      for (int r = 2 * split + half; r < p.Hq; r += step)
+      for (int r = mine; r < p.Hq; r += step)
         *reinterpret_cast<uint4*>(p.q_out + t * p.qo_tok + r * p.qo_head + 8 * l) =
             make_uint4(0, 0, 0, 0);
     return;
   }
-  Angles ang;
-  load_angles<MODE>(p.table + static_cast<size_t>(MODE != kNoRope ? pl.rope_pos : 0) * p.rot, p.rot,
-                    l, ang);
-
-  for (int base = 2 * split; base < nrows; base += kBatch * step) {
-    if (base != 2 * split) load(base);
-    #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      const int r0 = base + i * step;  // warp-uniform: the first half's row
-      if (r0 >= nrows) break;
-      const int r = r0 + half;
-      const int kind = r < p.Hq ? 0 : (r < p.Hq + p.Hkv ? 1 : 2);
-      const int h = kind == 0 ? r : (kind == 1 ? r - p.Hq : r - p.Hq - p.Hkv);
-      float x[8];
-      unpack8(raw[i], x);
-      if (p.qn.weight || p.kn.weight) {
-        float ss = 0.f;
-        #pragma unroll
-        for (int j = 0; j < 8; ++j) ss += x[j] * x[j];
-        #pragma unroll
-        for (int off = 1; off < 16; off <<= 1) ss += __shfl_xor_sync(kFull, ss, off);
-        const Norm& n = kind == 0 ? p.qn : p.kn;
-        if (kind < 2 && n.weight) {
-          const float f = rsqrtf(ss * (1.f / 128.f) + n.eps);
-          float wt[8];
-          load_weight(n, 8 * l, wt);
-          #pragma unroll
-          for (int j = 0; j < 8; ++j) x[j] = x[j] * f * wt[j];
-        }
-      }
-      rotate<MODE>(x, ang, p.rot, l, kind < 2);
-      if (r < nrows && kind == 0)
-        *reinterpret_cast<uint4*>(p.q_out + t * p.qo_tok + h * p.qo_head + 8 * l) = pack8(x);
-      if (!KV4) {
-        if (r < nrows && kind > 0 && page >= 0) {
-          __nv_bfloat16* c = static_cast<__nv_bfloat16*>(kind == 1 ? p.k_cache : p.v_cache);
-          *reinterpret_cast<uint4*>(
-              c + ((static_cast<size_t>(page) * p.tk.block_size + slot) * p.Hkv + h) * 128 + 8 * l) =
-              kind == 1 ? pack8(x) : raw[i];
-        }
-      } else if (r0 + 1 >= p.Hq) {  // warp-uniform: one of the two rows is K or V
-        unsigned short s16, c16;
-        const unsigned codes = quantise(x, group, s16, c16);
-        if (r < nrows && kind > 0 && page >= 0) {
-          const int ng = 128 / group, y = 8 * l / group, ti = slot % kv4::kTileTokens;
-          unsigned char* tile =
-              static_cast<unsigned char*>(kind == 1 ? p.k_cache : p.v_cache) +
-              ((static_cast<size_t>(page) * (p.tk.block_size / kv4::kTileTokens) +
-                slot / kv4::kTileTokens) * p.Hkv + h) * kv4::tile_bytes(group);
-          if (kind == 1) {
-            *reinterpret_cast<unsigned*>(tile + kv4::k_word(ti, l)) = codes;
-          } else {
-            *reinterpret_cast<unsigned short*>(tile + kv4::v_half(ti, 2 * l)) =
-                static_cast<unsigned short>(codes);
-            *reinterpret_cast<unsigned short*>(tile + kv4::v_half(ti, 2 * l + 1)) =
-                static_cast<unsigned short>(codes >> 16);
-          }
-          if (8 * l % group == 0) {
-            *reinterpret_cast<unsigned short*>(tile + kv4::scale_at(ti, y, ng)) = s16;
-            *reinterpret_cast<unsigned short*>(
-                tile + (kind == 1 ? kv4::k_centre_at(ti, y, ng) : kv4::v_centre_at(ti, y, ng))) =
-                c16;
-          }
-        }
-      }
+  const float* angles = p.table + static_cast<size_t>(MODE != kNoRope ? pl.rope_pos : 0) * p.rot;
+  turn_rows<MODE>(lay, q, p.q.head, mine, step, iters(mine, p.Hq), p.Hq, p.qn, angles, p.rot,
+                  p.q_out + t * p.qo_tok, p.qo_head);
+  const int kn = iters(k_first, p.Hkv), vn = iters(v_first, p.Hkv);
+  if (KV4) {
+    const size_t tile = (static_cast<size_t>(page) * (p.tk.block_size / kv4::kTileTokens) +
+                         slot / kv4::kTileTokens) * p.Hkv * kv4::tile_bytes(group);
+    unsigned char* const kt = page < 0 ? nullptr : static_cast<unsigned char*>(p.k_cache) + tile;
+    unsigned char* const vt = page < 0 ? nullptr : static_cast<unsigned char*>(p.v_cache) + tile;
+    const int ti = slot % kv4::kTileTokens;
+    quantise_rows<MODE, false>(k, p.k.head, k_first, step, kn, p.Hkv, p.kn, angles, p.rot, kt,
+                               ti, group);
+    quantise_rows<MODE, true>(v, p.v.head, v_first, step, vn, p.Hkv, p.kn, angles, p.rot, vt,
+                              ti, group);
+  } else if (page >= 0) {
+    const size_t row = (static_cast<size_t>(page) * p.tk.block_size + slot) * p.Hkv * 128;
+    turn_rows<MODE>(lay, k, p.k.head, k_first, step, kn, p.Hkv, p.kn, angles, p.rot,
+                    static_cast<__nv_bfloat16*>(p.k_cache) + row, 128);
+    __nv_bfloat16* const dst = static_cast<__nv_bfloat16*>(p.v_cache) + row + 8 * l;
+    for (int r = v_first; r < p.Hkv; r += kBatch * step) {
+      uint4 raw[kBatch];
+      #pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (r + i * step < p.Hkv) raw[i] = ld_stream(v + (r + i * step) * p.v.head + 8 * l);
+      #pragma unroll
+      for (int i = 0; i < kBatch; ++i)
+        if (r + i * step < p.Hkv) *reinterpret_cast<uint4*>(dst + (r + i * step) * 128) = raw[i];
     }
   }
 }
@@ -347,15 +519,16 @@ __global__ void __launch_bounds__(kThreads)
   constexpr int kRot = 64;
   const int lane = threadIdx.x & 31, l = lane & 7;
   const long long w = static_cast<long long>(blockIdx.x) * (kThreads / 32) + (threadIdx.x >> 5);
+  wait_for_stream();
   if (w >= static_cast<long long>(p.tk.rows) * p.nsplit) return;
   const int t = static_cast<int>(w / p.nsplit);
   const int split = static_cast<int>(w - static_cast<long long>(t) * p.nsplit);
   const int step = 4 * (p.nsplit - 1), first = 4 * (split - 1);
 
-  uint4 raw[kBatch];
+  uint4 raw[kMlaBatch];
   auto load = [&](int base) {
     #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
+    for (int i = 0; i < kMlaBatch; ++i) {
       const int h = base + i * step + (lane >> 3);
       raw[i] = h < p.h_q ? ld_stream(p.q_pe.data + t * p.q_pe.tok + h * p.q_pe.head + 8 * l)
                          : make_uint4(0, 0, 0, 0);
@@ -405,10 +578,12 @@ __global__ void __launch_bounds__(kThreads)
       #pragma unroll
       for (int off = 1; off < 32; off <<= 1) ss += __shfl_xor_sync(kFull, ss, off);
       const float f = rsqrtf(ss * (1.f / 512.f) + p.norm.eps);
-      load_weight(p.norm, 8 * lane, wt);
+      load_weight4(p.norm, 8 * lane, wt);
+      load_weight4(p.norm, 8 * lane + 4, wt + 4);
       #pragma unroll
       for (int j = 0; j < 8; ++j) a[j] = a[j] * f * wt[j];
-      load_weight(p.norm, 256 + 8 * lane, wt);
+      load_weight4(p.norm, 256 + 8 * lane, wt);
+      load_weight4(p.norm, 256 + 8 * lane + 4, wt + 4);
       #pragma unroll
       for (int j = 0; j < 8; ++j) b[j] = b[j] * f * wt[j];
       raw[0] = pack8(a);
@@ -425,10 +600,10 @@ __global__ void __launch_bounds__(kThreads)
     if (lane < 8) *reinterpret_cast<uint4*>(dst + 512 + 8 * l) = pack8(k);
     return;
   }
-  for (int base = first; base < p.h_q; base += kBatch * step) {
+  for (int base = first; base < p.h_q; base += kMlaBatch * step) {
     if (base != first) load(base);
     #pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
+    for (int i = 0; i < kMlaBatch; ++i) {
       if (base + i * step >= p.h_q) break;
       const int h = base + i * step + (lane >> 3);
       float x[8];
@@ -444,12 +619,12 @@ namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// Warps that fill the GPU once at half occupancy: with fewer, a token's heads
-// are spread over more warps.
+// Warps that run at once (four CTAs of eight on every SM): a call of fewer
+// tokens spreads each token's heads over as many as fit in that one wave.
 constexpr long long kFillWarps = 148 * 32;
 
 int pick_split(int rows, int most) {
-  long long n = (kFillWarps + rows - 1) / rows;
+  long long n = kFillWarps / rows;
   if (n > most) n = most;
   return n < 1 ? 1 : static_cast<int>(n);
 }
@@ -535,17 +710,14 @@ cudaError_t append_gqa(const kv_append_tokens* tokens, const kv_append_rope* rop
   const long long warps = static_cast<long long>(p.tk.rows) * p.nsplit;
   const long long grid = (warps + kThreads / 32 - 1) / (kThreads / 32);
   if (grid > INT_MAX) return cudaErrorInvalidValue;
-  const int g = static_cast<int>(grid);
-  if (group) {
-    if (mode == kNoRope) kv_append_gqa_kernel<kNoRope, true><<<g, kThreads, 0, stream>>>(p, group);
-    else if (mode == kHalves) kv_append_gqa_kernel<kHalves, true><<<g, kThreads, 0, stream>>>(p, group);
-    else kv_append_gqa_kernel<kPairs, true><<<g, kThreads, 0, stream>>>(p, group);
-  } else {
-    if (mode == kNoRope) kv_append_gqa_kernel<kNoRope, false><<<g, kThreads, 0, stream>>>(p, 0);
-    else if (mode == kHalves) kv_append_gqa_kernel<kHalves, false><<<g, kThreads, 0, stream>>>(p, 0);
-    else kv_append_gqa_kernel<kPairs, false><<<g, kThreads, 0, stream>>>(p, 0);
-  }
-  return cudaGetLastError();
+  using Kernel = void (*)(GqaParams, int);
+  const Kernel kernels[2][3] = {
+      {kv_append_gqa_kernel<kNoRope, false>, kv_append_gqa_kernel<kHalves, false>,
+       kv_append_gqa_kernel<kPairs, false>},
+      {kv_append_gqa_kernel<kNoRope, true>, kv_append_gqa_kernel<kHalves, true>,
+       kv_append_gqa_kernel<kPairs, true>}};
+  return launch_early(kernels[group ? 1 : 0][mode], static_cast<int>(grid), kThreads, 0, stream, p,
+                      group);
 }
 
 }  // namespace
@@ -614,11 +786,10 @@ cudaError_t kv_append_mla_launch(const kv_append_tokens* tokens, const kv_append
   const long long warps = static_cast<long long>(p.tk.rows) * p.nsplit;
   const long long grid = (warps + kThreads / 32 - 1) / (kThreads / 32);
   if (grid > INT_MAX) return cudaErrorInvalidValue;
-  const int g = static_cast<int>(grid);
-  if (mode == kNoRope) kv_append_mla_kernel<kNoRope><<<g, kThreads, 0, stream>>>(p);
-  else if (mode == kHalves) kv_append_mla_kernel<kHalves><<<g, kThreads, 0, stream>>>(p);
-  else kv_append_mla_kernel<kPairs><<<g, kThreads, 0, stream>>>(p);
-  return cudaGetLastError();
+  const auto kernel = mode == kNoRope   ? kv_append_mla_kernel<kNoRope>
+                      : mode == kHalves ? kv_append_mla_kernel<kHalves>
+                                        : kv_append_mla_kernel<kPairs>;
+  return gqa::launch_early(kernel, static_cast<int>(grid), kThreads, 0, stream, p);
 }
 
 int kv_append_get_status(int reset) {

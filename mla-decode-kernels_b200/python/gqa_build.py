@@ -28,7 +28,7 @@ EXT_PATH = os.path.join(BUILD_DIR, EXT_NAME + ".so")
 CU_SOURCES = ["gqa_scan.cu", "gqa_simt.cu", "gqa_api.cu", "gqa_cxx_abi.cu", "gqa_noalloc.cu",
               "mla_decode.cu", "dsa_decode.cu", "kv_append.cu", "kv4_decode.cu"]
 CU_HEADERS = ["gqa_internal.h", "gqa_ptx.cuh", "gqa_merge.cuh", "gqa_balance.cuh", "umma_ptx.cuh",
-              "device_once.h", "kv_tokens.cuh", "kv4_tile.cuh"]
+              "device_once.h", "launch_early.cuh", "kv_tokens.cuh", "kv4_tile.cuh"]
 PUBLIC_HEADERS = ["gqa_decode.h", "mla_decode.h", "dsa_decode.h", "kv_append.h", "kv4_decode.h"]
 EXT_SOURCES = ["gqa_decode_ext.cpp", "kv_cache_ext.cpp"]
 
