@@ -224,13 +224,17 @@ __device__ __forceinline__ uint32_t high_low(const float (&Q)[NG], int t) {
 
 struct Seg {
   int b, hg, row, S, s0, s1;
+  int cfirst, nparts;  // first CTA that holds a part of the row, and parts
 };
 
-// The CTA's share of the balanced schedule, as segments (one row, a range of
-// its tiles).  The copy warp and each planner keep their own, in shared memory.
+// The CTA's share of the schedule, as segments (one row, a range of its
+// tiles).  The copy warp and each planner keep their own.
+//   * Balanced (u == 0): tiles [g, g_end) of all rows' tiles in a line.
+//   * Parts (u > 0): rows cut into parts of u tiles, one part per CTA.
 struct Walk {
-  long long g, g_end, row0;
+  long long g, g_end, row0, T, E;
   int b, hg, S, L;
+  int u, part, parts;
 };
 
 __device__ __forceinline__ int req_len(const DecodeParams& p, int b) {
@@ -243,10 +247,11 @@ __device__ __forceinline__ int tiles_of(int len) {
   return static_cast<int>((static_cast<long long>(len) + kTileTokens - 1) / kTileTokens);
 }
 
-// The next segment of the walk; row_start = its row's first tile in the
-// schedule's order.  Every lane runs it on the same words.
-__device__ __forceinline__ bool next_seg(Walk* wp, const DecodeParams& p, Seg& s,
-                                         long long& row_start) {
+// The next segment of the walk.  Every lane runs it on the same words.
+// kOwners: with the row's parts (the copy warp does not need them, and their
+// divisions take time before the first copy).
+template <bool kOwners>
+__device__ __forceinline__ bool next_seg(Walk* wp, const DecodeParams& p, Seg& s) {
   Walk w = *wp;
   bool found = false;
   while (w.g < w.g_end) {
@@ -264,21 +269,30 @@ __device__ __forceinline__ bool next_seg(Walk* wp, const DecodeParams& p, Seg& s
       }
       continue;
     }
-    const long long e = min(w.g_end, re);
     s.b = w.b;
     s.hg = w.hg;
     s.row = w.b * p.pl.NHG + w.hg;
     s.S = w.S;
-    s.s0 = static_cast<int>(w.g - rs);
-    s.s1 = static_cast<int>(e - rs);
-    row_start = rs;
-    w.g = e;
+    if (w.u > 0) {
+      s.s0 = w.part * w.u;
+      s.s1 = min(w.L, s.s0 + w.u);
+      s.cfirst = static_cast<int>(blockIdx.x) - w.part;
+      s.nparts = w.parts;
+      w.g = w.g_end;
+    } else {
+      const long long e = min(w.g_end, re);
+      s.s0 = static_cast<int>(w.g - rs);
+      s.s1 = static_cast<int>(e - rs);
+      if (kOwners) {
+        s.cfirst = static_cast<int>(range_owner(rs, w.T, w.E));
+        s.nparts = static_cast<int>(range_owner(re - 1, w.T, w.E)) - s.cfirst + 1;
+      }
+      w.g = e;
+    }
     found = true;
     break;
   }
-  __syncwarp();
   *wp = w;
-  __syncwarp();
   return found;
 }
 
@@ -311,46 +325,83 @@ struct Record {
   int nparts;
 };
 
-// The CTA's range of the balanced schedule, by one warp alone (the same cut as
-// balanced_start's, whose result in `info` is used for large batches): every
-// lane takes a run of requests.
-constexpr int kWarpStart = 512;  // largest batch of which each helper warp makes its own start
-__device__ __forceinline__ void start_walk(const DecodeParams& p, const long long* info, Walk& walk,
-                                           long long& T, long long& E) {
+// The CTA's share, by one warp alone; every lane takes a run of requests.
+//
+// Balanced shares are equal but may reach over several rows, and each segment
+// costs a start and an end of its own, about as much as kSlack tiles.  Where
+// cutting every row into parts of u tiles gives no more than one part per CTA
+// with u at most kSlack above the balanced share - a few requests - that is
+// taken instead (four requests of up to 512 tokens: 14.0 -> 11.3 us).  For
+// batches above kWarpStart requests the CTA has made the balanced start in
+// `info` together.
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  // 64-bit division takes several times as long, on the way to the first copy
+  if (((a | b) >> 32) == 0)
+    return static_cast<unsigned>(a) / static_cast<unsigned>(b);
+  return a / b;
+}
+
+constexpr int kWarpStart = 512;
+constexpr int kSlack = 6;
+__device__ __forceinline__ void start_walk(const DecodeParams& p, const long long* info,
+                                           Walk& walk) {
   const int lane = threadIdx.x & 31, NHG = p.pl.NHG;
   Walk w;
-  w.hg = 0;
+  w.hg = w.u = w.part = w.parts = 0;
   if (p.B > kWarpStart) {
     w.g = info[0];
     w.g_end = info[1];
-    E = info[2];
+    w.E = info[2];
     w.b = static_cast<int>(info[3]);
     w.row0 = info[4] * NHG;
-    T = info[5];
+    w.T = info[5];
   } else {
     const int n = (p.B + 31) / 32;
     const int lo = min(p.B, lane * n), hi = min(p.B, lo + n);
-    long long local = 0;
-    #pragma unroll 4
-    for (int b = lo; b < hi; ++b) local += tiles_of(req_len(p, b));
-    long long x = local;
-    #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-      const long long y = __shfl_up_sync(kFull, x, off);
-      if (lane >= off) x += y;
+    // Of a request of L tiles: L, or its parts.
+    const auto weight = [&](int b, auto parts) -> long long {
+      const int L = tiles_of(req_len(p, b));
+      if constexpr (decltype(parts)::value) return (L + w.u - 1) / w.u;
+      return L;
+    };
+    long long local, x;  // of this lane's requests, and up to its last
+    const auto scan = [&](auto parts) {
+      local = 0;
+      #pragma unroll 4
+      for (int b = lo; b < hi; ++b) local += weight(b, parts);
+      x = local;
+      #pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const long long y = __shfl_up_sync(kFull, x, off);
+        if (lane >= off) x += y;
+      }
+      return __shfl_sync(kFull, x, 31) * NHG;
+    };
+    const long long grid = gridDim.x, spare = grid - static_cast<long long>(p.B) * NHG;
+    w.T = scan(std::false_type{});
+    if (spare > 0) {
+      const long long u = max(static_cast<long long>(kUnit), quotient(w.T + spare - 1, spare));
+      if (u * grid <= w.T + kSlack * grid) w.u = static_cast<int>(u);
     }
-    T = __shfl_sync(kFull, x, 31) * NHG;
-    E = range_parts(T, gridDim.x);
-    w.g = range_start(blockIdx.x, T, E);
-    w.g_end = range_start(blockIdx.x + 1LL, T, E);
+    if (w.u > 0) {
+      w.E = scan(std::true_type{});  // parts, at most grid
+      w.g = min(static_cast<long long>(blockIdx.x), w.E);
+      w.g_end = min(blockIdx.x + 1LL, w.E);
+    } else {
+      // (as range_parts and range_start)
+      w.E = max(1LL, min(grid, w.T / 2));
+      const long long c = blockIdx.x;
+      w.g = c >= w.E ? w.T : quotient(c * w.T, w.E);
+      w.g_end = c + 1 >= w.E ? w.T : quotient((c + 1) * w.T, w.E);
+    }
     long long before = x - local;
     const bool mine = w.g < w.g_end && w.g >= before * NHG && w.g < x * NHG;
     int b = lo;
     if (mine)
       for (; b < hi; ++b) {
-        const long long L = tiles_of(req_len(p, b));
-        if (w.g < (before + L) * NHG) break;
-        before += L;
+        const long long m = w.u > 0 ? weight(b, std::true_type{}) : weight(b, std::false_type{});
+        if (w.g < (before + m) * NHG) break;
+        before += m;
       }
     const unsigned who = __ballot_sync(kFull, mine);
     const int src = who ? __ffs(who) - 1 : 0;
@@ -359,8 +410,16 @@ __device__ __forceinline__ void start_walk(const DecodeParams& p, const long lon
   }
   w.S = w.g < w.g_end ? req_len(p, w.b) : 0;
   w.L = tiles_of(w.S);
+  if (w.u > 0 && w.g < w.g_end) {
+    w.parts = (w.L + w.u - 1) / w.u;
+    w.hg = static_cast<int>(w.g - w.row0) / w.parts;
+    w.part = static_cast<int>(w.g - w.row0) - w.hg * w.parts;
+    // one step inside the row, for next_seg
+    w.row0 = 0;
+    w.g = static_cast<long long>(w.hg) * w.L;
+    w.g_end = w.g + 1;
+  }
   walk = w;  // every lane the same
-  __syncwarp();
 }
 
 // A warp's softmax state: lane (g, t) holds heads 2 t and 2 t + 1 (n = 0, 1):
@@ -449,30 +508,27 @@ __device__ __forceinline__ void prepare_q(const DecodeParams& p, int b, int hg, 
 // planners), one segment ahead of the consumers, who prepare the first
 // segment's q themselves.
 template <int NG>
-__device__ __forceinline__ void plan_segments(const DecodeParams& p, Walk* walk, long long T,
-                                              long long E, int me, unsigned char* q_area,
-                                              Record* record, uint32_t filled, uint32_t read) {
+__device__ __forceinline__ void plan_segments(const DecodeParams& p, Walk* walk, int me,
+                                              unsigned char* q_area, Record* record,
+                                              uint32_t filled, uint32_t read) {
   const Plan& pl = p.pl;
   const int lane = threadIdx.x & 31;
   bool ok = true;  // the consumers still take records
   for (uint32_t n = 0;; ++n) {
     Seg s;
-    long long row_start;
-    const bool more = next_seg(walk, p, s, row_start);
+    const bool more = next_seg<true>(walk, p, s);
     if (ok && n > 0) ok = __all_sync(kFull, mbar_wait(read, (n - 1) & 1u));
     if (me == 0 && lane == 0) {
       Record r{};
       if (more) {
-        const int tiles = tiles_of(s.S);
-        const int cfirst = static_cast<int>(range_owner(row_start, T, E));
         r.valid = 1;
         r.b = s.b;
         r.hg = s.hg;
         r.row = s.row;
         r.tiles = s.s1 - s.s0;
         r.tokens = min(s.S - s.s0 * kTileTokens, r.tiles * kTileTokens);
-        r.nparts = static_cast<int>(range_owner(row_start + tiles - 1, T, E)) - cfirst + 1;
-        if (s.s0 == 0) p.row_info[s.row] = make_int2(cfirst, r.nparts);
+        r.nparts = s.nparts;
+        if (s.s0 == 0) p.row_info[s.row] = make_int2(s.cfirst, s.nparts);
       }
       if (ok) *record = r;
     }
@@ -509,7 +565,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ long long sh_info[8];
   __shared__ __align__(8) unsigned long long sh_full[kMaxSlots], sh_empty[kMaxSlots];
   __shared__ __align__(8) unsigned long long sh_seg[3];   // record filled, read; first q ready
-  __shared__ Walk sh_walk[1 + kPlanners];
   __shared__ Record sh_record;
   __shared__ uint32_t sh_given[kMaxWarps], sh_taken[kMaxWarps];  // meetings
 
@@ -535,17 +590,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     balanced_start(
         p.B, pl.NHG, [&](int b) -> long long { return tiles_of(req_len(p, b)); }, sh_warp, sh_info);
   __syncthreads();
-  Seg s;
-  long long row_start;
 
   if (warp >= kMaxWarps) {
     // -------------------------------- copies --------------------------------
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kHelperRegs));
-    Walk& walk = sh_walk[warp - kMaxWarps];
-    long long T, E;
-    start_walk(p, sh_info, walk, T, E);
+    Walk walk;  // the same in every lane
+    start_walk(p, sh_info, walk);
     if (warp > kMaxWarps) {
-      plan_segments<NG>(p, &walk, T, E, warp - kMaxWarps - 1, smem + pl.q_at, &sh_record,
+      plan_segments<NG>(p, &walk, warp - kMaxWarps - 1, smem + pl.q_at, &sh_record,
                         smem_u32(&sh_seg[0]), smem_u32(&sh_seg[1]));
       return;
     }
@@ -565,8 +617,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                                      tile / p.tiles_per_block)
                          : 0;
     };
-    Seg following;
-    bool more = next_seg(&walk, p, s, row_start);
+    Seg s, following;
+    bool more = next_seg<false>(&walk, p, s);
     int page = more ? look_up(s, s.s0) : 0;
     while (ok && more) {
       uint32_t cur = 0u;  // block * tiles per block + place in it
@@ -611,7 +663,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (st == s.s0) {
-          more = next_seg(&walk, p, following, row_start);
+          more = next_seg<false>(&walk, p, following);
           next_page = more ? look_up(following, following.s0) : 0;
         }
       }

@@ -111,6 +111,16 @@ def test_rows_cut_between_ctas(group, Hq, Hkv, bs, lens):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Hq,Hkv,bs", [(8, 2, 16), (16, 1, 64)])
+def test_equal_shares_that_cross_rows(Hq, Hkv, bs):
+    # too many rows of too uneven lengths for one part per CTA: shares that end
+    # and begin inside rows
+    lens = [2500, 3, 1700, 0, 1, 2499, 800] * 6
+    c = _case(lens, Hq, Hkv, bs, 64, seed=Hq)
+    _check(c, lens, _run(c, lens))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("B", [147, 512, 513, 700])
 def test_many_short_requests(B):
     # several rows per CTA, batches on both sides of the two ways to start the
