@@ -4,6 +4,7 @@
  * The operator is gqa_decode.h's, with K and V stored as 4-bit codes: the
  * `group` (32, 64 or 128) consecutive dims of one token and kv head share a
  * bf16 scale s and a bf16 centre c, and code n stands for s * (n - 8) + c.
+ * Scales are not negative.
  * The quantiser (kv_append_gqa_kv4_launch) takes, over the group's fp32
  * values x, s = (max - min) / 15 rounded up to bf16, c = min + 8 s rounded
  * to nearest bf16 and n = clamp(round((x - c) / s) + 8, 0, 15) (n = 8 where

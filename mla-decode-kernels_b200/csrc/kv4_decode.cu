@@ -17,7 +17,7 @@
 //     rounds (2^-12).  A q element below 2^-17 of its head's largest loses
 //     bits, 2^-25 of that largest at most.  The offset 8 is taken off by the
 //     centres' product, as the centre -8 s.
-//   * V: the same patterns, again raw; a byte's sum is 16 out' + out, which
+//   * V: the same four values, again raw; a byte's sum is 16 out' + out, which
 //     the end resolves.  The offset 8 joins the centres, through one product
 //     of the weights with a constant.  The raw sums grow with the context
 //     while what remains of them need not, and fp32 would lose the difference,
@@ -28,34 +28,47 @@
 // and moves only when one passes 2^15, so the common step takes no maximum
 // and rescales nothing.
 //
-// Layout (one persistent CTA per SM, the balanced schedule of gqa_balance.cuh):
-//   * up to 16 consumer warps, HG x NT x TS: kv head, 8 of its q heads, and
-//     every TS-th pair of tiles; the TS warps of a head keep their own state
-//     and meet at the end of a segment;
+// Layout (one persistent CTA per SM, the balanced schedule of gqa_balance.cuh,
+// or one part of a row per CTA for small batches):
+//   * up to 8 consumer warps, HG x NT x TS: kv head, 8 of its q heads, and
+//     every TS-th unit of 4 tiles; where TS > 1 the warps of a head keep their
+//     own state and meet at the end of a segment;
 //   * one copy warp: a row of HG kv heads is contiguous in the cache, so one
-//     cp.async.bulk brings a tile of all of them.  A ring slot holds K or V
-//     of 2 TS tiles;
+//     cp.async.bulk brings a tile of all of them (several tiles where a row is
+//     all heads and a block holds more).  A ring slot holds K or V of 4 TS
+//     tiles;
 //   * three planner warps: the next segment's record and its q fragments, made
 //     while the consumers work on the current one.
-// The consumers need more registers than 20 warps can share evenly, so the
-// copy and planner warps' group gives up most of its own.  A second kernel
+// The consumers need more registers than 12 warps can share evenly, so the
+// copy and planner warps' group gives up some of its own.  A second kernel
 // merges the rows that were cut between CTAs.
+//
+// Measured on one B200 (32 requests of 8192 tokens, 32 / 8 heads, group 64):
+// 61 us, 4.9 TB/s of cache, against 164 us from the bf16 cache and a floor of
+// 47 us.  About 11 us are the two launches, the first copies and the merge;
+// the stream alone, without the arithmetic, takes 43 us, and what remains is
+// arithmetic that does not hide behind it: 2 warps per scheduler issue in half
+// of its cycles (integer pipe 43 %, tensor pipe 32 %, 220 instructions per
+// 16-token tile and head, of which 64 unpack codes).  Sixteen warps of two
+// tiles at once (71 us), twelve warps (59 us on one long request, but 103 on
+// uneven batches for its narrower rows), and score and sum warps apart (66 us)
+// were slower; fp8 products are emulated for these warp-wide instructions.
 #include <cuda_fp16.h>
 #include <math.h>
 
 #include <algorithm>
-#include <type_traits>
 #include <climits>
 #include <cstdint>
+#include <type_traits>
 
 #include "device_once.h"
 #include "gqa_balance.cuh"
 #include "gqa_internal.h"
 #include "gqa_ptx.cuh"
-#include "launch_early.cuh"
 #include "kv4_decode.h"
 #include "kv4_tile.cuh"
 #include "kv_tokens.cuh"
+#include "launch_early.cuh"
 
 namespace gqa {
 namespace kv4 {
@@ -65,7 +78,7 @@ __device__ int g_kv4_status;
 namespace {
 
 constexpr unsigned kFull = 0xffffffffu;
-constexpr int kMaxWarps = 8;                // consumer warps
+constexpr int kMaxWarps = 8;                 // consumer warps
 constexpr int kUnit = 4;                     // tiles a warp works on at once
 constexpr int kMaxSlots = 16;
 constexpr int kPlanners = 3;
@@ -238,7 +251,7 @@ struct Walk {
 };
 
 __device__ __forceinline__ int req_len(const DecodeParams& p, int b) {
-  const int s = ld_nc_s32(p.seq_lens + b);
+  const int s = ld_plain(p.seq_lens + b);
   const long long cap = static_cast<long long>(p.max_blocks) * p.tiles_per_block * kTileTokens;
   return s < 0 ? 0 : static_cast<int>(min(static_cast<long long>(s), cap));
 }
@@ -325,6 +338,13 @@ struct Record {
   int nparts;
 };
 
+__device__ __forceinline__ long long quotient(long long a, long long b) {
+  // 64-bit division takes several times as long, on the way to the first copy
+  if (((a | b) >> 32) == 0)
+    return static_cast<unsigned>(a) / static_cast<unsigned>(b);
+  return a / b;
+}
+
 // The CTA's share, by one warp alone; every lane takes a run of requests.
 //
 // Balanced shares are equal but may reach over several rows, and each segment
@@ -334,13 +354,6 @@ struct Record {
 // taken instead (four requests of up to 512 tokens: 14.0 -> 11.3 us).  For
 // batches above kWarpStart requests the CTA has made the balanced start in
 // `info` together.
-__device__ __forceinline__ long long quotient(long long a, long long b) {
-  // 64-bit division takes several times as long, on the way to the first copy
-  if (((a | b) >> 32) == 0)
-    return static_cast<unsigned>(a) / static_cast<unsigned>(b);
-  return a / b;
-}
-
 constexpr int kWarpStart = 512;
 constexpr int kSlack = 6;
 __device__ __forceinline__ void start_walk(const DecodeParams& p, const long long* info,
@@ -450,7 +463,7 @@ __device__ __forceinline__ void prepare_q(const DecodeParams& p, int b, int hg, 
   uint32_t top = 0;  // largest |q| of the head, as bits
   #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint4 w = has ? __ldg(qrow + 4 * i + t) : make_uint4(0, 0, 0, 0);
+    const uint4 w = has ? ld_plain(qrow + 4 * i + t) : make_uint4(0, 0, 0, 0);
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
     #pragma unroll
     for (int k = 0; k < 4; ++k) top = max(top, max(u[k] & 0x7fffu, (u[k] >> 16) & 0x7fffu));
@@ -468,7 +481,7 @@ __device__ __forceinline__ void prepare_q(const DecodeParams& p, int b, int hg, 
   for (int y = 0; y < NG; ++y) Q[y] = R[y] = 0.f;
   #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint4 w = has ? __ldg(qrow + 4 * i + t) : make_uint4(0, 0, 0, 0);
+    const uint4 w = has ? ld_plain(qrow + 4 * i + t) : make_uint4(0, 0, 0, 0);
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
     float q[8];
     #pragma unroll
@@ -613,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool whole = pl.HG == p.Hkv;
     const auto look_up = [&](const Seg& q, int first) -> int {
       const int tile = first + lane;
-      return tile < q.s1 ? ld_nc_s32(p.block_table + static_cast<size_t>(q.b) * p.max_blocks +
+      return tile < q.s1 ? ld_plain(p.block_table + static_cast<size_t>(q.b) * p.max_blocks +
                                      tile / p.tiles_per_block)
                          : 0;
     };
@@ -868,7 +881,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           Scales<NG> sc;
           sc.load(vb + (i / kTileTokens) * tile_step + scale_at(i % kTileTokens, 0, NG));
           #pragma unroll
-          for (int y = 0; y < NG; ++y) sm = fmaxf(sm, sc[y]);
+          for (int y = 0; y < NG; ++y)
+            if (sc[y] < 1e38f) sm = fmaxf(sm, sc[y]);  // a group of infinities sets no range
         }
         #pragma unroll
         for (int off = 4; off < 32; off <<= 1) sm = fmaxf(sm, __shfl_xor_sync(kFull, sm, off));
@@ -1192,7 +1206,7 @@ __global__ void __launch_bounds__(256)
       pl.live = false;
     } else {
       const int lb = pl.pos / tk.block_size, slot = pl.pos - lb * tk.block_size;
-      int page = __ldg(tk.block_table + static_cast<size_t>(pl.b) * tk.max_blocks + lb);
+      int page = ld_plain(tk.block_table + static_cast<size_t>(pl.b) * tk.max_blocks + lb);
       if (static_cast<unsigned>(page) >= static_cast<unsigned>(tk.num_blocks)) {
         if (lane == 0) raise_status(kStatusBadPage);
         page = 0;
@@ -1206,7 +1220,7 @@ __global__ void __launch_bounds__(256)
   const int ck = k_word(ti, l), cv = v_half(ti, 2 * l), cv2 = v_half(ti, 2 * l + 1);
   const int sc = scale_at(ti, y, NG), zk = k_centre_at(ti, y, NG), zv = v_centre_at(ti, y, NG);
   const auto ld16 = [](const unsigned char* a) -> unsigned {
-    return __ldg(reinterpret_cast<const unsigned short*>(a));
+    return ld_plain(reinterpret_cast<const unsigned short*>(a));
   };
   // s (n - 8) + c: n as the last bits of 2^23 + n; the product is exact.
   const auto value = [](unsigned w, int i, unsigned s, unsigned c) {
@@ -1230,7 +1244,7 @@ __global__ void __launch_bounds__(256)
       if (pl.live && h < Hkv) {
         const unsigned char* a = kc + off + static_cast<size_t>(h) * kTile;
         const unsigned char* b = vc + off + static_cast<size_t>(h) * kTile;
-        wk[i] = __ldg(reinterpret_cast<const unsigned*>(a + ck));
+        wk[i] = ld_plain(reinterpret_cast<const unsigned*>(a + ck));
         wv[i] = ld16(b + cv) | ld16(b + cv2) << 16;
         sk[i] = ld16(a + sc);
         ok[i] = ld16(a + zk);

@@ -99,11 +99,12 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
 // Weights of dims d .. d + 3.
 __device__ __forceinline__ void load_weight4(const Norm& n, int d, float* w) {
   if (n.fp32) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(n.weight) + d));
+    const float4 a =
+        ld_plain(reinterpret_cast<const float4*>(static_cast<const float*>(n.weight) + d));
     w[0] = a.x; w[1] = a.y; w[2] = a.z; w[3] = a.w;
   } else {
     const uint2 a =
-        __ldg(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(n.weight) + d));
+        ld_plain(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(n.weight) + d));
     w[0] = __uint_as_float(a.x << 16); w[1] = __uint_as_float(a.x & 0xffff0000u);
     w[2] = __uint_as_float(a.y << 16); w[3] = __uint_as_float(a.y & 0xffff0000u);
   }
@@ -124,16 +125,16 @@ __device__ __forceinline__ void load_angles(const float* row, int rot, int l, An
     const int j = 8 * l < half ? 8 * l : 8 * l - half;
     #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float4 c = __ldg(reinterpret_cast<const float4*>(row + j) + i);
-      const float4 s = __ldg(reinterpret_cast<const float4*>(row + half + j) + i);
+      const float4 c = ld_plain(reinterpret_cast<const float4*>(row + j) + i);
+      const float4 s = ld_plain(reinterpret_cast<const float4*>(row + half + j) + i);
       const float sg = 8 * l < half ? -1.f : 1.f;
       a.c[4 * i] = c.x; a.c[4 * i + 1] = c.y; a.c[4 * i + 2] = c.z; a.c[4 * i + 3] = c.w;
       a.s[4 * i] = sg * s.x; a.s[4 * i + 1] = sg * s.y;
       a.s[4 * i + 2] = sg * s.z; a.s[4 * i + 3] = sg * s.w;
     }
   } else {
-    const float4 c = __ldg(reinterpret_cast<const float4*>(row + 4 * l));
-    const float4 s = __ldg(reinterpret_cast<const float4*>(row + half + 4 * l));
+    const float4 c = ld_plain(reinterpret_cast<const float4*>(row + 4 * l));
+    const float4 s = ld_plain(reinterpret_cast<const float4*>(row + half + 4 * l));
     a.c[0] = c.x; a.c[1] = c.y; a.c[2] = c.z; a.c[3] = c.w;
     a.s[0] = s.x; a.s[1] = s.y; a.s[2] = s.z; a.s[3] = s.w;
   }
@@ -276,8 +277,8 @@ __device__ __forceinline__ void make_turn(const Norm& n, const float* angles, in
   if (n.weight) load_weight4(n, lay.at0, w), load_weight4(n, lay.at1, w + 4);
   float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
   if (lay.on) {
-    c = __ldg(reinterpret_cast<const float4*>(angles + 4 * l));
-    s = __ldg(reinterpret_cast<const float4*>(angles + rot / 2 + 4 * l));
+    c = ld_plain(reinterpret_cast<const float4*>(angles + 4 * l));
+    s = ld_plain(reinterpret_cast<const float4*>(angles + rot / 2 + 4 * l));
   }
   const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
   #pragma unroll
@@ -451,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, 4)
   if (pl.live) {
     const int lb = pl.pos / p.tk.block_size;
     slot = pl.pos - lb * p.tk.block_size;
-    page = __ldg(p.tk.block_table + static_cast<size_t>(pl.b) * p.tk.max_blocks + lb);
+    page = ld_plain(p.tk.block_table + static_cast<size_t>(pl.b) * p.tk.max_blocks + lb);
     if (static_cast<unsigned>(page) >= static_cast<unsigned>(p.tk.num_blocks)) {
       bad = kStatusBadPage;
       page = -1;
@@ -564,7 +565,7 @@ __global__ void __launch_bounds__(kThreads)
   if (split == 0) {
     const int lb = pl.pos / p.tk.block_size;
     const int slot = pl.pos - lb * p.tk.block_size;
-    const int page = __ldg(p.tk.block_table + static_cast<size_t>(pl.b) * p.tk.max_blocks + lb);
+    const int page = ld_plain(p.tk.block_table + static_cast<size_t>(pl.b) * p.tk.max_blocks + lb);
     float k[8];
     unpack8(raw[2], k);
     rotate<MODE>(k, ang, kRot, l, true);

@@ -4,7 +4,7 @@
 
 #include <cstdint>
 
-#include "gqa_ptx.cuh"
+#include "launch_early.cuh"
 
 namespace gqa {
 
@@ -35,7 +35,7 @@ __device__ __forceinline__ int find_request(const int* cu, int batch, int t) {
     const int step = (n + 31) / 32;
     const int i = lo + (lane + 1) * step;  // sample: is cu[i] <= t?
     const bool in = (lane + 1) * step <= n;
-    const bool le = in && ld_nc_s32(cu + i) <= t;
+    const bool le = in && ld_plain(cu + i) <= t;
     const int c = __popc(__ballot_sync(0xffffffffu, le));  // samples passed
     lo += c * step;
     n = min(n - c * step, step - 1);
@@ -49,14 +49,14 @@ __device__ __forceinline__ Place find_place(const Tokens& k, int t) {
   int end = t + 1;  // rows of the request end here
   if (k.cu) {
     p.b = find_request(k.cu, k.batch, t);
-    if (p.b >= k.batch || t < ld_nc_s32(k.cu + p.b)) return p;
-    end = ld_nc_s32(k.cu + p.b + 1);
+    if (p.b >= k.batch || t < ld_plain(k.cu + p.b)) return p;
+    end = ld_plain(k.cu + p.b + 1);
   } else if (t >= k.batch) {
     return p;
   }
-  p.pos = ld_nc_s32(k.seq_lens + p.b) - (end - t);
+  p.pos = ld_plain(k.seq_lens + p.b) - (end - t);
   p.live = p.pos >= 0;
-  p.rope_pos = k.positions ? ld_nc_s32(k.positions + t) : p.pos;
+  p.rope_pos = k.positions ? ld_plain(k.positions + t) : p.pos;
   return p;
 }
 

@@ -18,6 +18,14 @@ __device__ __forceinline__ void wait_for_stream() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// A load of what an earlier kernel may have written.  Read-only (.nc) loads
+// are for data that stays the same while the kernel exists, and a kernel
+// launched early exists while the one before it still writes.
+template <class T>
+__device__ __forceinline__ T ld_plain(const T* p) {
+  return *p;
+}
+
 template <class... Params, class... Args>
 cudaError_t launch_early(void (*kernel)(Params...), int grid, int threads, size_t smem,
                          cudaStream_t stream, const Args&... args) {

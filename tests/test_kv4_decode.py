@@ -187,6 +187,27 @@ def test_long_context_stays_exact_to_the_tolerance():
 
 
 @pytest.mark.gpu
+def test_infinities_and_nan_stay_in_their_head():
+    # a scale that is infinite or NaN spoils the q heads of its request and kv
+    # head; the others keep their bits
+    lens = [300, 90]
+    c = _case(lens, 8, 2, 16, 32, seed=10)
+    clean = _run(c, lens)
+    k, v = c[1].clone(), c[2].clone()
+    scale = ref._byte_maps(32, True)[1]
+
+    def poison(cache, b, tok, head, y, bits):
+        tile = cache[int(c[3][b, tok // 16]), 0, head]
+        tile[scale[tok % 16, y]], tile[scale[tok % 16, y] + 1] = bits & 255, bits >> 8
+
+    poison(v, 0, 17, 0, 2, 0x7F80)   # infinity: dims 64 .. 95 of request 0, q heads 0 .. 3
+    poison(k, 1, 5, 1, 3, 0x7FC0)    # NaN: request 1, q heads 4 .. 7
+    got = _run((c[0], k, v, c[3]), lens)
+    assert not torch.isfinite(got[0, :4, 64:96]).any() and torch.isnan(got[1, 4:]).all()
+    assert torch.equal(got[0, 4:], clean[0, 4:]) and torch.equal(got[1, :4], clean[1, :4])
+
+
+@pytest.mark.gpu
 def test_equal_calls_give_equal_bits_and_out_is_written():
     lens = [3000, 1, 0, 700]
     c = _case(lens, 32, 8, 16, 64, seed=11)
