@@ -137,6 +137,14 @@ int kv4_group(const torch::Tensor& k_cache, const torch::Tensor& v_cache) {
   TORCH_CHECK(false, "the last dim of a 4-bit cache must be 1280, 1152 or 1088 (group 32, 64, 128)");
 }
 
+// Refuses overlaps that show from the tensors' bounds: of two views of one
+// buffer whose rows interleave nothing is said.
+void apart(const torch::Tensor& a, const torch::Tensor& b, const char* an, const char* bn) {
+  const auto o = at::get_overlap_status(a, b);
+  TORCH_CHECK(o != at::MemOverlapStatus::Full && o != at::MemOverlapStatus::Partial, an,
+              " must not overlap ", bn);
+}
+
 // The output of a rotated q: `out` after checks, or a new tensor.
 torch::Tensor rotated_out(const torch::Tensor& q, const OptTensor& out, const torch::Device& dev) {
   if (!out) return torch::empty(q.sizes(), q.options());
@@ -144,6 +152,14 @@ torch::Tensor rotated_out(const torch::Tensor& q, const OptTensor& out, const to
   TORCH_CHECK(out->sizes() == q.sizes(), "out must have q's shape");
   TORCH_CHECK(at::has_internal_overlap(*out) != at::MemOverlap::Yes,
               "out's elements must not share memory");
+  // Every element is read and written by one thread, so q's own place is fine.
+  if (out->numel() > 0 && out->data_ptr() == q.data_ptr()) {
+    TORCH_CHECK(used_stride(*out, 0) == used_stride(q, 0) &&
+                    used_stride(*out, 1) == used_stride(q, 1),
+                "out may be q, but not another view of its memory");
+  } else {
+    apart(*out, q, "out", "q");
+  }
   return *out;
 }
 
@@ -189,6 +205,10 @@ OptTensor gqa_append(OptTensor q, torch::Tensor k, torch::Tensor v, torch::Tenso
   long long out_tok = 0, out_head = 0;
   if (q) {
     result = rotated_out(*q, out, dev);
+    if (out) {
+      apart(*out, k, "out", "k");
+      apart(*out, v, "out", "v");
+    }
     if (rows) qh = heads(*q, true);
     out_tok = used_stride(*result, 0);
     out_head = used_stride(*result, 1);
@@ -243,6 +263,10 @@ OptTensor mla_append(torch::Tensor kv_c, torch::Tensor k_pe, torch::Tensor kv_ca
   long long out_tok = 0, out_head = 0;
   if (q_pe) {
     result = rotated_out(*q_pe, out, dev);
+    if (out) {
+      apart(*out, kv_c, "out", "kv_c");
+      apart(*out, k_pe, "out", "k_pe");
+    }
     if (rows) qh = heads(*q_pe, true);
     out_tok = used_stride(*result, 0);
     out_head = used_stride(*result, 1);
@@ -279,6 +303,7 @@ torch::Tensor gqa_decode_kv4(torch::Tensor q, torch::Tensor k_cache, torch::Tens
     TORCH_CHECK(out->is_cuda() && out->device() == dev && out->scalar_type() == torch::kBFloat16 &&
                     out->is_contiguous() && out->sizes() == q.sizes(),
                 "out must be a contiguous bf16 tensor of q's shape on the cache's device");
+    apart(*out, q, "out", "q");
   }
   const c10::cuda::CUDAGuard guard(dev);
   torch::Tensor o = out ? *out : torch::empty_like(q);

@@ -393,6 +393,76 @@ def test_a_serving_run_prompts_then_steps(group):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kv4", [False, True])
+def test_a_step_captured_with_copies_and_a_fork(kv4):
+    # kernels that may be launched early behind a copy, a memset and a join of
+    # two streams, all in one graph, replayed with other tokens each time
+    kv_append, kv4_decode = _modules()
+    import binding
+
+    gen = torch.Generator().manual_seed(22)
+    B, Hq, Hkv, bs = 40, 16, 4, 16
+    lens = torch.randint(1, 400, (B,), generator=gen).int()
+    table = torch.randperm(B * 26, generator=gen).int().view(B, 26).cuda()
+    cs = kv_append.rope_cos_sin(401, 128)
+
+    def caches():
+        g = torch.Generator().manual_seed(23)
+        if not kv4:
+            return [torch.randn(B * 26, bs, Hkv, 128, generator=g).bfloat16().cuda() for _ in range(2)]
+        c = kv4_decode.new_cache(B * 26, bs, Hkv)
+        rows = [torch.randn(B * 400, Hkv, 128, generator=g).bfloat16().cuda() for _ in range(2)]
+        kv_append.gqa_append_kv4(None, *rows, *c, table, torch.full((B,), 400, dtype=torch.int32, device="cuda"),
+                                 cu_seqlens=torch.arange(0, B * 400 + 1, 400, dtype=torch.int32, device="cuda"))
+        return c
+
+    append = kv_append.gqa_append_kv4 if kv4 else kv_append.gqa_append
+    decode = kv4_decode.gqa_decode_kv4 if kv4 else binding.gqa_decode
+    sl = torch.zeros(B, dtype=torch.int32, device="cuda")
+    qkv = torch.zeros(B, Hq + 2 * Hkv, 128, device="cuda").bfloat16()
+    q, k, v = qkv.split([Hq, Hkv, Hkv], 1)
+    mine = caches()
+    src, host_lens = torch.zeros_like(qkv), lens.cuda()
+    side = torch.cuda.Stream()
+
+    def step():
+        sl.zero_()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            sl.add_(host_lens)
+        qkv.copy_(src)
+        torch.cuda.current_stream().wait_stream(side)
+        qo = append(q, k, v, *mine, table, sl, cs)
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            one = decode(qo, *mine, table, sl, SCALE)
+        if not kv4:  # binding.gqa_decode's calls share a workspace
+            torch.cuda.current_stream().wait_stream(side)
+        two = decode(qo, *mine, table, sl, -SCALE)
+        torch.cuda.current_stream().wait_stream(side)
+        return one, two
+
+    step()
+    torch.cuda.synchronize()
+    mine = [t.copy_(c) for t, c in zip(mine, caches())]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step()
+    plain = caches()
+    for _ in range(4):
+        rows = torch.randn(qkv.shape, generator=gen).bfloat16().cuda()
+        src.copy_(rows)
+        host_lens.copy_(lens)
+        g.replay()
+        torch.cuda.synchronize()
+        qo = append(*rows.split([Hq, Hkv, Hkv], 1), *plain, table, lens.cuda(), cs)
+        torch.cuda.synchronize()
+        for o, s in zip(got, (SCALE, -SCALE)):
+            assert torch.equal(o, decode(qo, *plain, table, lens.cuda(), s))
+        lens = lens % 400 + 1
+
+
+@pytest.mark.gpu
 def test_a_latent_step_appends_and_attends():
     kv_append, _ = _modules()
     import mla_decode
@@ -448,6 +518,8 @@ def test_refusals():
             kv4_decode.gqa_decode_kv4(*a)
     with pytest.raises(RuntimeError, match="out must be"):
         kv4_decode.gqa_decode_kv4(*good, out=torch.zeros(2, 8, 64, device="cuda").bfloat16())
+    with pytest.raises(RuntimeError, match="must not overlap q"):
+        kv4_decode.gqa_decode_kv4(*good, out=q)
     with pytest.raises(ValueError, match="rows"):
         kv4_decode.gqa_gather_kv4(k, v, bt, sl, torch.zeros(3, dtype=torch.int32, device="cuda"))
     assert kv4_decode.gqa_decode_kv4(q[:0], k, v, bt[:0], sl[:0], SCALE).shape == (0, 8, 128)

@@ -494,6 +494,15 @@ def test_refusals():
     ]:
         with pytest.raises(RuntimeError, match=match):
             call(**kw)
+    buf = torch.zeros(6 * 4 * 128, device="cuda").bfloat16()
+    out, behind = buf[:1024].view(2, 4, 128), buf[512:1024].view(2, 2, 128)
+    for match, kw in [("overlap k", dict(i=1, t=behind, out=out)), ("overlap v", dict(i=2, t=behind, out=out)),
+                      ("overlap q", dict(i=0, t=buf[512:1536].view(2, 4, 128), out=out)),
+                      ("another view", dict(i=0, t=buf.view(6, 4, 128)[::3], out=out))]:
+        with pytest.raises(RuntimeError, match=match):
+            call(**kw)
+    row = torch.zeros(1, 4, 128, device="cuda").bfloat16()  # the stride of a single row says nothing
+    kv_append.gqa_append(row.as_strided((1, 4, 128), (8, 128, 1)), k[:1], v[:1], kc, vc, bt[:1], sl[:1], out=row)
     wrong = torch.zeros(3, 1, 2, 1200, dtype=torch.uint8, device="cuda")
     with pytest.raises(RuntimeError, match="last dim of a 4-bit cache"):
         kv_append.gqa_append_kv4(q, k, v, wrong, wrong.clone(), bt, sl)
