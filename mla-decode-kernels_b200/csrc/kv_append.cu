@@ -14,6 +14,13 @@
 // keeps its angles, multiplied by the norm's weights, in registers over all
 // the heads it takes; small calls give every warp fewer heads instead, down
 // to one row per half warp, so that one token's heads run side by side.
+//
+// Measured on one B200 (64 / 8 heads with norms): 4 prompts of 8192 tokens
+// 223 us, 6.1 TB/s of a copy's 6.45; a step of 128 tokens 4.9 us, one token
+// of 32 / 8 heads 2.8 us, both a launch and the chain request -> page -> row.
+// Into the 4-bit cache, 16400 tokens of 32 / 8 heads take 96 us: the codes'
+// arithmetic, DRAM at 55 %.  Latent rows: 8200 tokens with 64 heads 27 us,
+// 5.7 TB/s.
 #include <cuda_bf16.h>
 #include <math.h>
 
