@@ -81,6 +81,8 @@ constexpr unsigned kFull = 0xffffffffu;
 constexpr int kMaxWarps = 8;                 // consumer warps
 constexpr int kUnit = 4;                     // tiles a warp works on at once
 constexpr int kMaxSlots = 16;
+constexpr int kWarpStart = 512;  // requests that one warp's start of the schedule takes
+constexpr int kSlack = 6;        // tiles' worth of time of a segment's start and end
 constexpr int kPlanners = 3;
 constexpr int kThreads = (kMaxWarps + 1 + kPlanners) * 32;  // consumers, copy warp, planners
 // Registers: 384 threads at 168 are launched; 256 consumer threads at 208 and
@@ -102,6 +104,7 @@ struct Plan {
   int NT;       // 8-head column tiles of a part
   int HG, NHG;  // kv heads per row, rows per request (Hkv / HG * QP)
   int TS, warps;
+  int pad;      // tiles that a row counts longer than it is, for its start and end
   int meet;     // the first step of a meeting: the power of two below TS
   int slot_tiles, slot_bytes, nslots;
   int q_at, box_at, smem;  // bytes: q fragments, meeting boxes, all dynamic shared memory
@@ -242,11 +245,13 @@ struct Seg {
 
 // The CTA's share of the schedule, as segments (one row, a range of its
 // tiles).  The copy warp and each planner keep their own.
-//   * Balanced (u == 0): tiles [g, g_end) of all rows' tiles in a line.
+//   * Balanced (u == 0): places [g, g_end) of all rows in a line, where a row
+//     takes `pad` places, for what its start costs, and then its tiles.
 //   * Parts (u > 0): rows cut into parts of u tiles, one part per CTA.
 struct Walk {
   long long g, g_end, row0, T, E;
   int b, hg, S, L;
+  int pad;
   int u, part, parts;
 };
 
@@ -260,6 +265,8 @@ __device__ __forceinline__ int tiles_of(int len) {
   return static_cast<int>((static_cast<long long>(len) + kTileTokens - 1) / kTileTokens);
 }
 
+__device__ __forceinline__ int places_of(int tiles, int pad) { return tiles ? tiles + pad : 0; }
+
 // The next segment of the walk.  Every lane runs it on the same words.
 // kOwners: with the row's parts (the copy warp does not need them, and their
 // divisions take time before the first copy).
@@ -268,11 +275,12 @@ __device__ __forceinline__ bool next_seg(Walk* wp, const DecodeParams& p, Seg& s
   Walk w = *wp;
   bool found = false;
   while (w.g < w.g_end) {
-    const long long rs = w.row0 + static_cast<long long>(w.hg) * w.L, re = rs + w.L;
+    const int places = places_of(w.L, w.pad);
+    const long long rs = w.row0 + static_cast<long long>(w.hg) * places, re = rs + places;
     if (w.g >= re) {
       if (++w.hg == p.pl.NHG) {
         w.hg = 0;
-        w.row0 += static_cast<long long>(p.pl.NHG) * w.L;
+        w.row0 += static_cast<long long>(p.pl.NHG) * places;
         if (++w.b >= p.B) {
           w.g = w.g_end;
           break;
@@ -280,6 +288,12 @@ __device__ __forceinline__ bool next_seg(Walk* wp, const DecodeParams& p, Seg& s
         w.S = req_len(p, w.b);
         w.L = tiles_of(w.S);
       }
+      continue;
+    }
+    const long long t0 = rs + w.pad;  // the first tile's place
+    const long long e = min(w.g_end, re);
+    if (e <= t0) {
+      w.g = e;
       continue;
     }
     s.b = w.b;
@@ -293,11 +307,10 @@ __device__ __forceinline__ bool next_seg(Walk* wp, const DecodeParams& p, Seg& s
       s.nparts = w.parts;
       w.g = w.g_end;
     } else {
-      const long long e = min(w.g_end, re);
-      s.s0 = static_cast<int>(w.g - rs);
-      s.s1 = static_cast<int>(e - rs);
+      s.s0 = static_cast<int>(max(w.g, t0) - t0);
+      s.s1 = static_cast<int>(e - t0);
       if (kOwners) {
-        s.cfirst = static_cast<int>(range_owner(rs, w.T, w.E));
+        s.cfirst = static_cast<int>(range_owner(t0, w.T, w.E));
         s.nparts = static_cast<int>(range_owner(re - 1, w.T, w.E)) - s.cfirst + 1;
       }
       w.g = e;
@@ -347,20 +360,21 @@ __device__ __forceinline__ long long quotient(long long a, long long b) {
 
 // The CTA's share, by one warp alone; every lane takes a run of requests.
 //
-// Balanced shares are equal but may reach over several rows, and each segment
-// costs a start and an end of its own, about as much as kSlack tiles.  Where
-// cutting every row into parts of u tiles gives no more than one part per CTA
-// with u at most kSlack above the balanced share - a few requests - that is
-// taken instead (four requests of up to 512 tokens: 14.0 -> 11.3 us).  For
-// batches above kWarpStart requests the CTA has made the balanced start in
-// `info` together.
-constexpr int kWarpStart = 512;
-constexpr int kSlack = 6;
+// Balanced shares may reach over several rows, and each segment costs a start
+// and an end of its own, about as much as kSlack tiles of each of a head's
+// warps: a row counts that much longer than it is (64 requests of 64 to 16384
+// tokens 67 -> 58.5 us, 700 of 4 to 4096 163 -> 119; with 4 and 10 instead of
+// 6: 61 and 59, 127 and 115).  Where cutting every row into parts of u tiles
+// gives no more than one part per CTA with u at most kSlack above the balanced
+// share - a few requests - that is taken instead (four requests of up to 512
+// tokens: 14.0 -> 11.3 us).  For batches above kWarpStart requests the CTA has
+// made the balanced start in `info` together.
 __device__ __forceinline__ void start_walk(const DecodeParams& p, const long long* info,
                                            Walk& walk) {
   const int lane = threadIdx.x & 31, NHG = p.pl.NHG;
   Walk w;
   w.hg = w.u = w.part = w.parts = 0;
+  w.pad = p.pl.pad;
   if (p.B > kWarpStart) {
     w.g = info[0];
     w.g_end = info[1];
@@ -371,17 +385,22 @@ __device__ __forceinline__ void start_walk(const DecodeParams& p, const long lon
   } else {
     const int n = (p.B + 31) / 32;
     const int lo = min(p.B, lane * n), hi = min(p.B, lo + n);
-    // Of a request of L tiles: L, or its parts.
+    // Of a request of L tiles: its places, or its parts.
     const auto weight = [&](int b, auto parts) -> long long {
       const int L = tiles_of(req_len(p, b));
       if constexpr (decltype(parts)::value) return (L + w.u - 1) / w.u;
-      return L;
+      return places_of(L, w.pad);
     };
     long long local, x;  // of this lane's requests, and up to its last
+    int rows = 0;        // its requests with tokens
     const auto scan = [&](auto parts) {
       local = 0;
       #pragma unroll 4
-      for (int b = lo; b < hi; ++b) local += weight(b, parts);
+      for (int b = lo; b < hi; ++b) {
+        const long long m = weight(b, parts);
+        local += m;
+        if constexpr (!decltype(parts)::value) rows += m > 0;
+      }
       x = local;
       #pragma unroll
       for (int off = 1; off < 32; off <<= 1) {
@@ -393,10 +412,13 @@ __device__ __forceinline__ void start_walk(const DecodeParams& p, const long lon
     const long long grid = gridDim.x, spare = grid - static_cast<long long>(p.B) * NHG;
     w.T = scan(std::false_type{});
     if (spare > 0) {
-      const long long u = max(static_cast<long long>(kUnit), quotient(w.T + spare - 1, spare));
-      if (u * grid <= w.T + kSlack * grid) w.u = static_cast<int>(u);
+      const long long T =
+          w.T - static_cast<long long>(__reduce_add_sync(kFull, rows)) * NHG * w.pad;
+      const long long u = max(static_cast<long long>(kUnit), quotient(T + spare - 1, spare));
+      if (u * grid <= T + kSlack * grid) w.u = static_cast<int>(u);
     }
     if (w.u > 0) {
+      w.pad = 0;
       w.E = scan(std::true_type{});  // parts, at most grid
       w.g = min(static_cast<long long>(blockIdx.x), w.E);
       w.g_end = min(blockIdx.x + 1LL, w.E);
@@ -601,7 +623,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   wait_for_stream();
   if (p.B > kWarpStart)
     balanced_start(
-        p.B, pl.NHG, [&](int b) -> long long { return tiles_of(req_len(p, b)); }, sh_warp, sh_info);
+        p.B, pl.NHG,
+        [&](int b) -> long long { return places_of(tiles_of(req_len(p, b)), pl.pad); }, sh_warp,
+        sh_info);
   __syncthreads();
 
   if (warp >= kMaxWarps) {
@@ -1289,6 +1313,7 @@ int make_plan(int Hq, int Hkv, int group, Plan* p) {
       best = d * ts;
       p->HG = d;
       p->TS = ts;
+      p->pad = kSlack * ts;
     }
   }
   p->NHG = Hkv / p->HG * p->QP;
