@@ -44,13 +44,13 @@
 // merges the rows that were cut between CTAs.
 //
 // Measured on one B200 (32 requests of 8192 tokens, 32 / 8 heads, group 64):
-// 61 us, 4.9 TB/s of cache, against 164 us from the bf16 cache and a floor of
+// 61 us, 5.0 TB/s of cache, against 164 us from the bf16 cache and a floor of
 // 47 us.  About 11 us are the two launches, the first copies and the merge;
 // the stream alone, without the arithmetic, takes 43 us, and what remains is
 // arithmetic that does not hide behind it: 2 warps per scheduler issue in half
 // of its cycles (integer pipe 43 %, tensor pipe 32 %, 220 instructions per
 // 16-token tile and head, of which 64 unpack codes).  Sixteen warps of two
-// tiles at once (71 us), twelve warps (59 us on one long request, but 103 on
+// tiles at once (71 us), twelve warps (59 us on one long request, but slower on
 // uneven batches for its narrower rows), and score and sum warps apart (66 us)
 // were slower; fp8 products are emulated for these warp-wide instructions.
 #include <cuda_fp16.h>
@@ -1210,7 +1210,7 @@ __global__ void __launch_bounds__(256) kv4_merge_kernel(const MergeParams p) {
 // Read-back: a warp on one token, half a warp per kv head, 8 dims per lane;
 // nsplit warps share a token's heads where there are few tokens.
 // Bound by latency for few tokens (32: 2.4 us) and by its writes for many
-// (16400 tokens of 8 heads: 21 us, 3.9 TB/s read and written).
+// (16400 tokens of 8 heads: 21 us, 4.2 TB/s read and written).
 template <int NG>
 __global__ void __launch_bounds__(256)
     kv4_gather_kernel(const __grid_constant__ Tokens tk, const unsigned char* kc,

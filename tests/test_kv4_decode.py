@@ -121,6 +121,17 @@ def test_equal_shares_that_cross_rows(Hq, Hkv, bs):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("Hq,Hkv,B", [(8, 8, 160), (4, 2, 160), (1, 1, 600)])
+def test_shares_that_end_at_a_row_s_start(Hq, Hkv, B):
+    # rows of one tile and rows that are cut, in turn: shares that end inside
+    # what a row counts for its start
+    gen = torch.Generator().manual_seed(B + Hq)
+    lens = [int(2 ** (10.5 * float(x))) - 1 for x in torch.rand(B, generator=gen)]
+    c = _case(lens, Hq, Hkv, 16, 128, seed=B)
+    _check(c, lens, _run(c, lens))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("B", [147, 512, 513, 700])
 def test_many_short_requests(B):
     # several rows per CTA, batches on both sides of the two ways to start the
