@@ -303,8 +303,9 @@ __device__ __forceinline__ void make_turn(const Norm& n, const float* angles, in
 // (rows may differ between the halves, `iters` may not).  At dst rows are
 // dst_stride apart.
 template <int MODE>
-__device__ __forceinline__ void turn_rows(const Lay<MODE>& lay, const __nv_bfloat16* src, long long stride, int first,
-                                          int step, int iters, int count, const Norm& n,
+__device__ __forceinline__ void turn_rows(const Lay<MODE>& lay, const __nv_bfloat16* src,
+                                          long long stride, int first, int step, int iters,
+                                          int count, const Norm& n,
                                           const float* angles, int rot, __nv_bfloat16* dst,
                                           long long dst_stride) {
   const int l = threadIdx.x & 15;
