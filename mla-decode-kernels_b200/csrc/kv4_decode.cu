@@ -13,10 +13,12 @@
 //     stands, and a whole byte (16 n' + n) 2^-24.  q enters in fp16, divided
 //     by a power of two per head so that its largest element is in [1, 2)
 //     (and by 16 more where it meets 16 n); where n' comes with n in one byte,
-//     n meets q - q' / 16 instead, which is the only one of four that fp16
-//     rounds (2^-12).  A q element below 2^-17 of its head's largest loses
-//     bits, 2^-25 of that largest at most.  The offset 8 is taken off by the
-//     centres' product, as the centre -8 s.
+//     n meets q - q' / 16 instead, which fp16 rounds by up to 2^-11 of it.
+//     The others it holds exactly except far below the head's largest: a q
+//     that meets 16 n or a byte loses bits below 2^-13 of that, 2^-21 at most,
+//     one that meets n below 2^-17, 2^-25 at most.  The offset 8 is taken off
+//     by the centres' product, as the centre -8 s times the sum of the rounded
+//     values, so that codes of 8 cancel whatever was rounded.
 //   * V: the same four values, again raw; a byte's sum is 16 out' + out, which
 //     the end resolves.  The offset 8 joins the centres, through one product
 //     of the weights with a constant.  The raw sums grow with the context
@@ -498,7 +500,7 @@ __device__ __forceinline__ void prepare_q(const DecodeParams& p, int b, int hg, 
       p.scale_log2 * 16777216.f * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
   dst[18 * 32] = __float_as_uint(__shfl_sync(kFull, up, 8 * t));
   dst[19 * 32] = __float_as_uint(__shfl_sync(kFull, up, 8 * t + 4));
-  float Q[NG], R[NG];  // sums of q, and of what its roundings leave
+  float Q[NG], R[NG];  // sums of q, and of q as rounded, which the codes meet
   #pragma unroll
   for (int y = 0; y < NG; ++y) Q[y] = R[y] = 0.f;
   #pragma unroll
@@ -512,15 +514,19 @@ __device__ __forceinline__ void prepare_q(const DecodeParams& p, int b, int hg, 
       q[2 * k + 1] = __uint_as_float(u[k] & 0xffff0000u) * down;
     }
     const float h = 0.0625f;
-    const uint32_t d = pack_half2(q[2] - q[3] * h, q[6] - q[7] * h);
-    dst[(4 * i) * 32] = pack_half2(q[0], q[4]);
-    dst[(4 * i + 1) * 32] = pack_half2(q[1] * h, q[5] * h);
-    dst[(4 * i + 2) * 32] = d;
-    dst[(4 * i + 3) * 32] = pack_half2(q[3] * h, q[7] * h);
-    const float2 df = __half22float2(*reinterpret_cast<const __half2*>(&d));
-    const float rest = q[0] + q[4] + q[1] + q[5] + q[3] + q[7];
-    float a = rest + (q[2] + q[6]);
-    float b = rest + (df.x + q[3] * h) + (df.y + q[7] * h);
+    const uint32_t f[4] = {pack_half2(q[0], q[4]), pack_half2(q[1] * h, q[5] * h),
+                           pack_half2(q[2] - q[3] * h, q[6] - q[7] * h),
+                           pack_half2(q[3] * h, q[7] * h)};
+    float r[4];  // sums of the pairs as rounded
+    #pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      dst[(4 * i + k) * 32] = f[k];
+      const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&f[k]));
+      r[k] = x.x + x.y;
+    }
+    // a code of 8 everywhere is 8 b: n meets f[0], 16 n f[1], a byte f[3] and n f[2]
+    float a = (q[0] + q[4] + q[1] + q[5]) + (q[2] + q[6] + q[3] + q[7]);
+    float b = r[0] + 16.f * r[1] + r[2] + 17.f * r[3];
     #pragma unroll
     for (int off = 1; off < 4; off <<= 1) {
       a += __shfl_xor_sync(kFull, a, off);
