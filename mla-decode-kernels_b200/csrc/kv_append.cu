@@ -213,15 +213,19 @@ __device__ __forceinline__ unsigned quantise(const float (&x)[8], int group, uns
   const float s = want != want ? want
                                : __uint_as_float((__float_as_uint(want) + 0xffffu) & 0xffff0000u);
   const __nv_bfloat16 cb = __float2bfloat16(__fadd_rn(lo, __fmul_rn(8.f, s)));
-  const float c = __bfloat162float(cb);
+  // Where 1 / s or a quotient's remainder would leave fp32's normal numbers,
+  // 2^64 times everything has the same quotients.  x - c is up x - up c in one
+  // rounding, for up = 1 too, so this costs nothing per value.
+  const float up = s < 0x1p-100f && s > 0.f ? 0x1p64f : 1.f;
+  const float step = s * up, at = -__bfloat162float(cb) * up;
   float inv;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(step));
   if (s == 0.f) inv = 0.f;  // the group is one value up to the rounding of c: n = 8
   unsigned w = 0;
   #pragma unroll
   for (int i = 6; i >= 0; i -= 2) {
-    const int n0 = __float2int_rn(quotient(__fsub_rn(x[i], c), s, inv));
-    const int n1 = __float2int_rn(quotient(__fsub_rn(x[i + 1], c), s, inv));
+    const int n0 = __float2int_rn(quotient(__fmaf_rn(x[i], up, at), step, inv));
+    const int n1 = __float2int_rn(quotient(__fmaf_rn(x[i + 1], up, at), step, inv));
     // clamped to [-8, 7] and put below what is there
     asm("cvt.pack.sat.s4.s32.b32 %0, %1, %2, %0;" : "+r"(w) : "r"(n1), "r"(n0));
   }
