@@ -147,11 +147,10 @@ __device__ __forceinline__ void load_angles(const float* row, int rot, int l, An
   }
 }
 
-// Rotates x (dims 8 l .. of a head) where `on`.  Every lane of the warp must
-// call it: in the half layout the pair's other element is rot / 16 lanes
-// away.  Products and sums are rounded one by one, in the formula's order.
+// Rotates x (dims 8 l .. of a head).  Every lane of the warp must call it: in
+// the half layout the pair's other element is rot / 16 lanes away.  Products and sums are rounded one by one, in the formula's order.
 template <int MODE>
-__device__ __forceinline__ void rotate(float (&x)[8], const Angles& a, int rot, int l, bool on) {
+__device__ __forceinline__ void rotate(float (&x)[8], const Angles& a, int rot, int l) {
   if (MODE == kNoRope) return;
   const bool in = 8 * l < rot;
   if (MODE == kHalves) {
@@ -160,9 +159,9 @@ __device__ __forceinline__ void rotate(float (&x)[8], const Angles& a, int rot, 
     #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float o = __shfl_sync(kFull, x[i], from);
-      if (on && in) x[i] = __fadd_rn(__fmul_rn(x[i], a.c[i]), __fmul_rn(o, a.s[i]));
+      if (in) x[i] = __fadd_rn(__fmul_rn(x[i], a.c[i]), __fmul_rn(o, a.s[i]));
     }
-  } else if (on && in) {
+  } else if (in) {
     #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float u = x[2 * i], v = x[2 * i + 1];
@@ -407,7 +406,7 @@ __device__ __forceinline__ void quantise_rows(const __nv_bfloat16* src, long lon
           #pragma unroll
           for (int j = 0; j < 8; ++j) x[j] = x[j] * f * wt[j];
         }
-        rotate<MODE>(x, ang, rot, l, true);
+        rotate<MODE>(x, ang, rot, l);
       }
       unsigned short s16, c16;
       const unsigned codes = quantise(x, group, s16, c16);
@@ -580,7 +579,7 @@ __global__ void __launch_bounds__(kThreads)
     const int page = ld_plain(p.tk.block_table + static_cast<size_t>(pl.b) * p.tk.max_blocks + lb);
     float k[8];
     unpack8(raw[2], k);
-    rotate<MODE>(k, ang, kRot, l, true);
+    rotate<MODE>(k, ang, kRot, l);
     if (p.norm.weight) {
       float a[8], b[8], wt[8];
       unpack8(raw[0], a);
@@ -621,7 +620,7 @@ __global__ void __launch_bounds__(kThreads)
       const int h = base + i * step + (lane >> 3);
       float x[8];
       unpack8(raw[i], x);
-      rotate<MODE>(x, ang, kRot, l, true);
+      rotate<MODE>(x, ang, kRot, l);
       if (h < p.h_q)
         *reinterpret_cast<uint4*>(p.q_out + t * p.qo_tok + h * p.qo_head + 8 * l) = pack8(x);
     }
