@@ -76,8 +76,8 @@ typedef struct kv_append_norm {
 
 /* q [rows, Hq, 128] -> q_out (same strides kind), k and v [rows, Hkv, 128] ->
  * k_cache and v_cache [num_blocks, block_size, Hkv, 128].  q.data NULL: only
- * K and V.  q_out may be q itself.  Values are held in fp32 between the load
- * and one rounding to bf16 at the store. */
+ * K and V.  q_out may be q itself; caches that overlap are refused.  Values
+ * are held in fp32 between the load and one rounding to bf16 at the store. */
 cudaError_t kv_append_gqa_launch(const kv_append_tokens* tokens, const kv_append_rope* rope,
                                  kv_append_heads q, kv_append_heads k, kv_append_heads v,
                                  kv_append_norm q_norm, kv_append_norm k_norm, gqa_bf16* q_out,

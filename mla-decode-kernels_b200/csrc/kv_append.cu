@@ -148,7 +148,8 @@ __device__ __forceinline__ void load_angles(const float* row, int rot, int l, An
 }
 
 // Rotates x (dims 8 l .. of a head).  Every lane of the warp must call it: in
-// the half layout the pair's other element is rot / 16 lanes away.  Products and sums are rounded one by one, in the formula's order.
+// the half layout the pair's other element is rot / 16 lanes away.  Products
+// and sums are rounded one by one, in the formula's order.
 template <int MODE>
 __device__ __forceinline__ void rotate(float (&x)[8], const Angles& a, int rot, int l) {
   if (MODE == kNoRope) return;
@@ -641,6 +642,12 @@ int pick_split(int rows, int most) {
   return n < 1 ? 1 : static_cast<int>(n);
 }
 
+// Whether [a, a + bytes) and [b, b + bytes) share memory.
+bool overlap(const void* a, const void* b, unsigned long long bytes) {
+  const auto x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return (x > y ? x - y : y - x) < bytes;
+}
+
 cudaError_t check_tokens(const kv_append_tokens* a, Tokens* t) {
   if (!a) return cudaErrorInvalidValue;
   if (a->rows < 0 || a->batch < 0 || a->max_blocks <= 0 || a->num_blocks <= 0 || a->block_size <= 0)
@@ -713,6 +720,9 @@ cudaError_t append_gqa(const kv_append_tokens* tokens, const kv_append_rope* rop
   }
   if (!k_cache || !v_cache) return cudaErrorInvalidValue;
   if (!aligned16(k_cache) || !aligned16(v_cache)) return cudaErrorMisalignedAddress;
+  const unsigned long long row_bytes = group ? kv4::tile_bytes(group) / kv4::kTileTokens : 256;
+  if (overlap(k_cache, v_cache, row_bytes * p.tk.num_blocks * p.tk.block_size * Hkv))
+    return cudaErrorInvalidValue;
   p.Hq = q.data ? Hq : 0;
   p.Hkv = Hkv;
   p.k_cache = k_cache;

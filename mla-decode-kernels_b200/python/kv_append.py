@@ -102,8 +102,8 @@ def gqa_append(q, k, v, k_cache, v_cache, block_table, seq_lens, cos_sin=None, c
     q [rows, Hq, 128] (None: only K and V are handled, None is returned), k and
     v [rows, Hkv, 128] bf16, caches [num_blocks, block_size, Hkv, 128] bf16;
     q_weight and k_weight [128] bf16 or fp32 (None: no norm): y = x *
-    rsqrt(mean(x^2) + eps) * weight over each head.  out may be q itself, and else must not
-    overlap q, k or v."""
+    rsqrt(mean(x^2) + eps) * weight over each head.  out may be q itself, and
+    else must not overlap q, k, v or the caches, nor k_cache v_cache."""
     return _ext.gqa_append(q, k, v, k_cache, v_cache, block_table, seq_lens, cos_sin, cu_seqlens,
                            positions, interleaved, q_weight, k_weight, eps, out, False)
 

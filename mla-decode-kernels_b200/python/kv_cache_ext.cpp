@@ -178,6 +178,7 @@ OptTensor gqa_append(OptTensor q, torch::Tensor k, torch::Tensor v, torch::Tenso
                 "k_cache and v_cache must have the same shape and device");
     TORCH_CHECK(k_cache.size(3) == 128, "k_cache must be [num_blocks, block_size, Hkv, 128]");
   }
+  apart(k_cache, v_cache, "k_cache", "v_cache");
   const torch::Device dev = k_cache.device();
   const int64_t block_size = kv4 ? 16 * k_cache.size(1) : k_cache.size(1);
   const int64_t Hkv = k_cache.size(2);
@@ -208,6 +209,8 @@ OptTensor gqa_append(OptTensor q, torch::Tensor k, torch::Tensor v, torch::Tenso
     if (out) {
       apart(*out, k, "out", "k");
       apart(*out, v, "out", "v");
+      apart(*out, k_cache, "out", "k_cache");
+      apart(*out, v_cache, "out", "v_cache");
     }
     if (rows) qh = heads(*q, true);
     out_tok = used_stride(*result, 0);
@@ -266,6 +269,7 @@ OptTensor mla_append(torch::Tensor kv_c, torch::Tensor k_pe, torch::Tensor kv_ca
     if (out) {
       apart(*out, kv_c, "out", "kv_c");
       apart(*out, k_pe, "out", "k_pe");
+      apart(*out, kv_cache, "out", "kv_cache");
     }
     if (rows) qh = heads(*q_pe, true);
     out_tok = used_stride(*result, 0);
@@ -304,6 +308,8 @@ torch::Tensor gqa_decode_kv4(torch::Tensor q, torch::Tensor k_cache, torch::Tens
                     out->is_contiguous() && out->sizes() == q.sizes(),
                 "out must be a contiguous bf16 tensor of q's shape on the cache's device");
     apart(*out, q, "out", "q");
+    apart(*out, k_cache, "out", "k_cache");
+    apart(*out, v_cache, "out", "v_cache");
   }
   const c10::cuda::CUDAGuard guard(dev);
   torch::Tensor o = out ? *out : torch::empty_like(q);

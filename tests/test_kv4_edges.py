@@ -81,3 +81,67 @@ def test_codes_of_the_smallest_and_largest_values(group):
         top = g.abs().amax(-1) + 2.0 ** -133
         tol = (s / 2 + 2.0 ** -7 * (top + s) + 2.0 ** -133).repeat_interleave(group, -1)
         assert torch.all((got.cpu().double() - want).abs() <= tol)
+
+
+def _c_append():
+    """kv_append_gqa_launch and _kv4_launch as functions of the caches' addresses
+    (one row and head, 3 pages of 16 tokens); nothing is read before the refusal."""
+    import ctypes
+
+    import binding
+    import test_kv_append as t
+
+    lib = ctypes.CDLL(binding.LIB_PATH)
+    P, L, I = ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int
+    head = [P, P, t._Heads, t._Heads, t._Heads, t._Norm, t._Norm, P, L, L, I, P, P, I, I]
+    lib.kv_append_gqa_launch.argtypes = head + [P]
+    lib.kv_append_gqa_kv4_launch.argtypes = head + [I, P]
+    ok = 4096
+    tok = t._Tokens(block_table=ok, seq_lens=ok, rows=1, batch=1, max_blocks=1, num_blocks=3, block_size=16)
+    rope = t._Rope(table=None)
+    row = t._Heads(data=ok, token_stride=128, head_stride=128)
+    args = [ctypes.byref(tok), ctypes.byref(rope), t._Heads(None, 0, 0), row, row, t._Norm(None, 0, 0.0),
+            t._Norm(None, 0, 0.0), None, 0, 0, 0]
+    return (lambda k, v: lib.kv_append_gqa_launch(*args, k, v, 0, 1, None),
+            lambda k, v: lib.kv_append_gqa_kv4_launch(*args, k, v, 0, 1, 64, None))
+
+
+def test_c_appends_refuse_caches_that_overlap():
+    bf16, kv4 = _c_append()
+    at = 1 << 20
+    for call, size in ((bf16, 3 * 16 * 256), (kv4, 3 * 1152)):
+        for k, v in ((at, at), (at, at + 16), (at + size - 16, at), (at, at + size - 16)):
+            assert call(k, v) == 1, (k, v)  # cudaErrorInvalidValue
+
+
+@pytest.mark.gpu
+def test_caches_and_outputs_that_overlap_are_refused():
+    kv_append, kv4_decode = _modules()
+    pages = torch.zeros(6, 16, 2, 128, dtype=torch.bfloat16, device="cuda")
+    tiles = torch.zeros(6, 1, 2, 1152, dtype=torch.uint8, device="cuda")
+    x = torch.ones(2, 2, 128, dtype=torch.bfloat16, device="cuda")
+    table = torch.tensor([[0], [1]], dtype=torch.int32, device="cuda")
+    sl = torch.ones(2, dtype=torch.int32, device="cuda")
+    for call, c in ((kv_append.gqa_append, pages), (kv_append.gqa_append_kv4, tiles)):
+        for k, v in ((c, c), (c[:4], c[2:]), (c[3:], c[1:4])):
+            with pytest.raises(RuntimeError, match="k_cache must not overlap v_cache"):
+                call(None, x, x, k, v, table, sl)
+        call(None, x, x, c[:3], c[3:], table, sl)  # neighbours in one buffer
+        assert torch.any(c[0] != 0) and torch.any(c[3] != 0)
+    assert torch.equal(pages[0, 0], x[0]) and torch.equal(pages[4, 0], x[1])
+    assert not pages[2].any() and not pages[5].any() and not tiles[2].any() and not tiles[5].any()
+    inside = pages.view(-1, 2, 128)[:2]
+    with pytest.raises(RuntimeError, match="out must not overlap k_cache"):
+        kv_append.gqa_append(x, x, x, pages[:3], pages[3:], table, sl, out=inside)
+    with pytest.raises(RuntimeError, match="out must not overlap v_cache"):
+        kv_append.gqa_append(x, x, x, pages[3:], pages[:3], table, sl, out=inside)
+    inside = tiles.view(torch.bfloat16).flatten()[:512].view(2, 2, 128)
+    for k, v, name in ((tiles[:3], tiles[3:], "k_cache"), (tiles[3:], tiles[:3], "v_cache")):
+        with pytest.raises(RuntimeError, match="out must not overlap " + name):
+            kv4_decode.gqa_decode_kv4(x, k, v, table, sl, 1.0, out=inside)
+    latent = torch.zeros(2, 64, 1, 576, dtype=torch.bfloat16, device="cuda")
+    q = torch.ones(2, 2, 64, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(RuntimeError, match="out must not overlap kv_cache"):
+        kv_append.mla_append(torch.ones(2, 512, device="cuda").bfloat16(), q[:, 0], latent, table, sl, q_pe=q,
+                             out=latent.flatten()[:256].view(2, 2, 64))
+    assert kv_append.get_status(True) == 0 and kv4_decode.get_status(True) == 0
