@@ -45,6 +45,8 @@ def gqa_gather_kv4(k_cache, v_cache, block_table, seq_lens, cu_seqlens=None, row
     gqa_append_kv4 takes them; rows without a token are zero.  rows is the
     output's size (without cu_seqlens: one row per request, its last token)."""
     if cu_seqlens is None:
+        if rows not in (None, seq_lens.shape[0]):
+            raise ValueError("without cu_seqlens there is one row per request")
         rows = seq_lens.shape[0]
     elif rows is None:
         raise ValueError("rows is needed with cu_seqlens")

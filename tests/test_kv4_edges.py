@@ -145,3 +145,13 @@ def test_caches_and_outputs_that_overlap_are_refused():
         kv_append.mla_append(torch.ones(2, 512, device="cuda").bfloat16(), q[:, 0], latent, table, sl, q_pe=q,
                              out=latent.flatten()[:256].view(2, 2, 64))
     assert kv_append.get_status(True) == 0 and kv4_decode.get_status(True) == 0
+
+
+def test_read_back_refuses_rows_that_it_would_not_return():
+    _, kv4_decode = _modules()
+    k, v = kv4_decode.new_cache(2, 16, 1, device="cpu")
+    table, sl = torch.zeros(2, 1).int(), torch.ones(2).int()
+    with pytest.raises(ValueError, match="one row per request"):
+        kv4_decode.gqa_gather_kv4(k, v, table, sl, rows=3)
+    with pytest.raises(RuntimeError, match="must be a CUDA tensor"):  # the right number passes on
+        kv4_decode.gqa_gather_kv4(k, v, table, sl, rows=2)
