@@ -155,3 +155,15 @@ def test_read_back_refuses_rows_that_it_would_not_return():
         kv4_decode.gqa_gather_kv4(k, v, table, sl, rows=3)
     with pytest.raises(RuntimeError, match="must be a CUDA tensor"):  # the right number passes on
         kv4_decode.gqa_gather_kv4(k, v, table, sl, rows=2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("Hq,Hkv", [(65, 1), (100, 1), (146, 2), (127, 1)])
+def test_groups_of_q_heads_cut_into_unequal_parts(Hq, Hkv):
+    # more than 64 q heads per kv head are two rows of the schedule, the second
+    # with fewer heads, down to warps that have none
+    import test_kv4_decode as t
+
+    for lens in ([1, 0, 40, 300], [900, 17] * 80):
+        c = t._case(lens, Hq, Hkv, 16, 64, seed=Hq + len(lens))
+        t._check(c, lens, t._run(c, lens))
