@@ -6,7 +6,9 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <climits>
+#include <cstdlib>
 #include <tuple>
 
 #include "kv4_decode.h"
@@ -145,20 +147,51 @@ void apart(const torch::Tensor& a, const torch::Tensor& b, const char* an, const
               " must not overlap ", bn);
 }
 
+// Whether rows of heads a and b [rows, heads, dim] of equal strides, as slices
+// of one projection have, share memory; with a itself: whether two of its
+// heads do.  Head (t, h) of a and (t', h') of b are delta + dt ts + dh hs
+// elements apart, and share memory where that is less than dim.
+bool rows_meet(const torch::Tensor& a, const torch::Tensor& b) {
+  const int64_t T = a.size(0), dim = a.size(2), ts = used_stride(a, 0);
+  const int64_t hs = a.size(1) > 1 ? a.stride(1) : used_stride(b, 1);
+  const int64_t delta = (reinterpret_cast<intptr_t>(b.data_ptr()) -
+                         reinterpret_cast<intptr_t>(a.data_ptr())) / a.element_size();
+  const bool self = a.is_same(b);
+  for (int64_t dh = 1 - a.size(1); dh < b.size(1); ++dh) {
+    const int64_t at = delta + dh * hs;
+    // the closest is this dt or one next to it
+    const int64_t near = ts > 0 ? std::clamp(-at / ts, 1 - T, T - 1) : 0;
+    for (int64_t dt = std::max(near - 1, 1 - T); dt <= std::min(near + 1, T - 1); ++dt)
+      if (!(self && dt == 0 && dh == 0) && std::abs(at + dt * ts) < dim) return true;
+  }
+  return false;
+}
+
+// apart() for an output and an input of rows of heads, exact where their
+// strides are equal.
+void rows_apart(const torch::Tensor& a, const torch::Tensor& b, const char* an, const char* bn) {
+  if (a.numel() == 0 || b.numel() == 0) return;
+  if (used_stride(a, 0) == used_stride(b, 0) &&
+      (a.size(1) == 1 || b.size(1) == 1 || a.stride(1) == b.stride(1))) {
+    TORCH_CHECK(!rows_meet(a, b), an, " must not overlap ", bn);
+  } else {
+    apart(a, b, an, bn);
+  }
+}
+
 // The output of a rotated q: `out` after checks, or a new tensor.
 torch::Tensor rotated_out(const torch::Tensor& q, const OptTensor& out, const torch::Device& dev) {
   if (!out) return torch::empty(q.sizes(), q.options());
   check_rows(*out, dev, q.size(2), 3, "out");
   TORCH_CHECK(out->sizes() == q.sizes(), "out must have q's shape");
-  TORCH_CHECK(at::has_internal_overlap(*out) != at::MemOverlap::Yes,
-              "out's elements must not share memory");
+  TORCH_CHECK(out->numel() == 0 || !rows_meet(*out, *out), "out's elements must not share memory");
   // Every element is read and written by one thread, so q's own place is fine.
   if (out->numel() > 0 && out->data_ptr() == q.data_ptr()) {
     TORCH_CHECK(used_stride(*out, 0) == used_stride(q, 0) &&
                     used_stride(*out, 1) == used_stride(q, 1),
                 "out may be q, but not another view of its memory");
   } else {
-    apart(*out, q, "out", "q");
+    rows_apart(*out, q, "out", "q");
   }
   return *out;
 }
@@ -207,8 +240,8 @@ OptTensor gqa_append(OptTensor q, torch::Tensor k, torch::Tensor v, torch::Tenso
   if (q) {
     result = rotated_out(*q, out, dev);
     if (out) {
-      apart(*out, k, "out", "k");
-      apart(*out, v, "out", "v");
+      rows_apart(*out, k, "out", "k");
+      rows_apart(*out, v, "out", "v");
       apart(*out, k_cache, "out", "k_cache");
       apart(*out, v_cache, "out", "v_cache");
     }

@@ -167,3 +167,44 @@ def test_groups_of_q_heads_cut_into_unequal_parts(Hq, Hkv):
     for lens in ([1, 0, 40, 300], [900, 17] * 80):
         c = t._case(lens, Hq, Hkv, 16, 64, seed=Hq + len(lens))
         t._check(c, lens, t._run(c, lens))
+
+
+@pytest.mark.gpu
+def test_outputs_that_overlap_between_strides_are_refused():
+    # slices of one projection whose bounds interleave: refused where heads
+    # share memory, taken where they only lie between one another
+    kv_append, _ = _modules()
+    table = torch.tensor([[0], [1], [2]], dtype=torch.int32, device="cuda")
+    sl = torch.ones(3, dtype=torch.int32, device="cuda")
+    kc, vc = torch.zeros(2, 3, 16, 2, 128, dtype=torch.bfloat16, device="cuda")
+    cs = kv_append.rope_cos_sin(4, 128)
+    qkv = torch.randn(3, 16, 128, generator=torch.Generator().manual_seed(0)).bfloat16().cuda()
+    q, k, v = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:8]
+
+    def call(out, q=q):
+        return kv_append.gqa_append(q, k, v, kc, vc, table, sl, cs, out=out)
+
+    for out, what in ((qkv[:, 1:5], "q"), (qkv[:, 5:9], "k"), (qkv[:, 7:11], "v"),
+                      (qkv.flatten()[4 * 128 - 8:].as_strided((3, 4, 128), (2048, 128, 1)), "q"),
+                      (qkv.as_strided((3, 4, 128), (2048, 64, 1), 8 * 128), "memory"),
+                      (qkv.as_strided((3, 4, 128), (384, 128, 1), 8 * 128), "memory"),
+                      (qkv.as_strided((3, 4, 128), (8, 512, 1), 8 * 128), "memory")):
+        before = qkv.clone()
+        with pytest.raises(RuntimeError, match="overlap " + what if what != "memory" else "share memory"):
+            call(out)
+        assert torch.equal(qkv, before)
+    want = call(None)
+    row = torch.zeros(3, 5, 128, dtype=torch.bfloat16, device="cuda")
+    for out in (qkv[:, 8:12], qkv[:, 8:16:2], row[:, 1:], torch.zeros(4, 3, 128, device="cuda").bfloat16().transpose(0, 1),
+                torch.zeros(3000, device="cuda").bfloat16().as_strided((3, 4, 128), (640, 256, 1))):
+        assert torch.equal(call(out), want)
+    assert torch.equal(call(q.clone()), want)
+    assert torch.equal(call(q), want)  # in place, last: q is rotated now
+    latent = torch.zeros(3, 64, 1, 576, dtype=torch.bfloat16, device="cuda")
+    full = torch.randn(3, 2, 192, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    args = (torch.ones(3, 512, device="cuda").bfloat16(), torch.ones(3, 64, device="cuda").bfloat16(), latent, table, sl)
+    with pytest.raises(RuntimeError, match="overlap q"):
+        kv_append.mla_append(*args, q_pe=full[..., 64:128], out=full[..., 72:136])
+    kv_append.mla_append(*args, q_pe=full[..., 64:128], out=full[..., 128:])
+    assert torch.equal(full[..., 128:], full[..., 64:128])  # no table: a copy
+    assert kv_append.get_status(True) == 0
