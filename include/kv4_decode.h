@@ -8,7 +8,11 @@
  * The quantiser (kv_append_gqa_kv4_launch) takes, over the group's fp32
  * values x, s = (max - min) / 15 rounded up to bf16, c = min + 8 s rounded
  * to nearest bf16 and n = clamp(round((x - c) / s) + 8, 0, 15) (n = 8 where
- * s = 0).  A group that holds a NaN or an infinity reads back as NaN.
+ * s = 0).  No code is clipped but for c's rounding to bf16, which shifts
+ * a group's codes where |c| is large against its range (mean 20, deviation
+ * 0.3: errors of up to a step; mean 100: three).  A group that holds a NaN or
+ * an infinity, or whose range passes fp32's, reads back as NaN; in the decode
+ * it spoils all dims of the request's q heads of its kv head.
  *
  * K and V caches are uint8 [num_blocks, block_size / 16, Hkv, tile], tile =
  * 1024 + 64 * (128 / group) bytes: one tile is 16 tokens of one kv head,
@@ -46,7 +50,8 @@ size_t kv4_decode_workspace_bytes(int B, int Hq, int Hkv, int group);
 
 /* out[b, h] = softmax_t(q[b, h] . K[t] * scale) @ V[t] over t < seq_lens[b]
  * (0 for a request without tokens); q and out bf16 [B, Hq, 128], block_table
- * int32 [B, max_blocks], seq_lens int32 [B].  block_size a multiple of 16,
+ * int32 [B, max_blocks], seq_lens int32 [B], lengths past the block table's
+ * row count as its end and negative ones as 0.  block_size a multiple of 16,
  * q, out, caches and workspace 16-byte aligned.  A block id outside
  * [0, num_blocks) sets bit 1 of kv4_decode_get_status and reads block 0.
  * Calls that may overlap on the GPU must not share a workspace. */
@@ -69,9 +74,9 @@ cudaError_t kv4_gather_launch(const unsigned char* k_cache, const unsigned char*
                               int block_size, int max_blocks, int num_blocks,
                               cudaStream_t stream);
 
-/* Device status word of the 4-bit cache's kernels (bit 0: a bounded wait
- * gave up, bit 1: block id out of range, bit 3: position out of range);
- * reset clears it.  Synchronises the device; negative: the read failed. */
+/* Status word of the 4-bit cache's kernels on the current device (bit 0: a
+ * bounded wait gave up, bit 1: block id out of range, bit 3: position out of
+ * range); reset clears it.  Synchronises the device; negative: the read failed. */
 int kv4_decode_get_status(int reset);
 
 #ifdef __cplusplus

@@ -107,8 +107,8 @@ cudaError_t kv_append_mla_launch(const kv_append_tokens* tokens, const kv_append
                                  int zero_skipped, gqa_bf16* kv_cache, int h_q,
                                  cudaStream_t stream);
 
-/* Device status word of the append kernels: bit 1 (value 2) = a block id
- * outside [0, num_blocks): that token's K and V were not written; bit 3
+/* Status word of the append kernels on the current device: bit 1 (value 2) = a
+ * block id outside [0, num_blocks): that token's K and V were not written; bit 3
  * (value 8) = a position outside the block table's row or the rotation
  * table: that row was treated as holding no token.  reset clears it.
  * Synchronises the device; negative: the read failed. */

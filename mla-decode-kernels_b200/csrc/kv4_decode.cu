@@ -24,7 +24,16 @@
 //     of the weights with a constant.  The raw sums grow with the context
 //     while what remains of them need not, and fp32 would lose the difference,
 //     so every kFold units the centres' sum is folded into them.
-//     The weights p_t s_ty are rounded to fp16, 2^-11.
+// Roundings, half a step each, beside those of q above: the weights p_t s_ty
+// that meet codes to fp16, 2^-11; the weights p_t that meet centres to bf16,
+// 2^-8, the widest (their range is not fp16's: p_t is 2^9 over a scale); the
+// sums of q that meet centres and -8 s to two bf16 parts, 2^-17; ex2.approx,
+// 2^-22.  Everything else is summed in fp32.  Against 64 bits the output is off
+// by 0.0018-0.0020 (relative rms), of which its own rounding to bf16 is 0.0017.
+// A scale that is NaN or infinite spoils all dims of its request's q heads of
+// that kv head (the product with -8 has zeros that meet it); V's scales count
+// in full from 1e-18 to 1e30, smaller ones lose bits in fp16 and from 1e32 on
+// the products overflow.
 // The softmax reference M of a head is no running maximum but any value that
 // keeps the fp16 weights in range: it is set so that the largest p s is 2^9
 // and moves only when one passes 2^15, so the common step takes no maximum
@@ -46,12 +55,16 @@
 // merges the rows that were cut between CTAs.
 //
 // Measured on one B200 (32 requests of 8192 tokens, 32 / 8 heads, group 64):
-// 61 us, 5.0 TB/s of cache, against 164 us from the bf16 cache and a floor of
-// 47 us.  About 11 us are the two launches, the first copies and the merge;
-// the stream alone, without the arithmetic, takes 43 us, and what remains is
-// arithmetic that does not hide behind it: 2 warps per scheduler issue in half
-// of its cycles (integer pipe 43 %, tensor pipe 32 %, 220 instructions per
-// 16-token tile and head, of which 64 unpack codes).  Sixteen warps of two
+// 59.5 us in a CUDA graph (64 us call by call), 5.1 TB/s of cache, against 159
+// us from the bf16 cache and a floor of 47 us.  About 11 us are the two
+// launches, the first copies and the merge; the stream alone, without the
+// arithmetic, takes 43 us, and what remains is latency between the dependent
+// steps of a unit that does not hide behind it: 2 warps per scheduler issue in
+// 43 % of its cycles (integer pipe 40 %, tensor pipe 30 %, 220 instructions per
+// 16-token tile and head, of which 64 unpack codes).  More than 8 q heads per
+// kv head unpack every code once per 8 of them: 112, 213 and 410 us for 16, 32
+// and 64 of each kv head (the bf16 cache: 312, 615 and 1209).  Group 32 (70.5
+// us) spills 40 to 56 bytes at its 168 registers.  Sixteen warps of two
 // tiles at once (71 us), twelve warps (59 us on one long request, but slower on
 // uneven batches for its narrower rows), and score and sum warps apart (66 us)
 // were slower; fp8 products are emulated for these warp-wide instructions.
@@ -1215,8 +1228,10 @@ __global__ void __launch_bounds__(256) kv4_merge_kernel(const MergeParams p) {
 
 // Read-back: a warp on one token, half a warp per kv head, 8 dims per lane;
 // nsplit warps share a token's heads where there are few tokens.
-// Bound by latency for few tokens (32: 2.4 us) and by its writes for many
-// (16400 tokens of 8 heads: 21 us, 4.2 TB/s read and written).
+// Bound by latency for few tokens (32: 2.4 us) and for many (16400 tokens of 8
+// heads: 21 us against 14 of bytes) by its instructions, two- and four-byte
+// loads with scales and centres loaded anew in every lane: issue 62 %, integer
+// pipe 59 %, DRAM 1.3 TB/s.
 template <int NG>
 __global__ void __launch_bounds__(256)
     kv4_gather_kernel(const __grid_constant__ Tokens tk, const unsigned char* kc,

@@ -16,11 +16,12 @@
 // to one row per half warp, so that one token's heads run side by side.
 //
 // Measured on one B200 (64 / 8 heads with norms): 4 prompts of 8192 tokens
-// 223 us, 6.1 TB/s of a copy's 6.45; a step of 128 tokens 4.9 us, one token
+// 224 us, 6.1 TB/s of a copy's 6.45; a step of 128 tokens 4.9 us, one token
 // of 32 / 8 heads 2.8 us, both a launch and the chain request -> page -> row.
-// Into the 4-bit cache, 16400 tokens of 32 / 8 heads take 96 us: the codes'
-// arithmetic, DRAM at 55 %.  Latent rows: 8200 tokens with 64 heads 27 us,
-// 5.7 TB/s.
+// Into the 4-bit cache, 16400 tokens of 32 / 8 heads take 97 us against 57 of
+// bytes: 71 % of issue slots, integer pipe 53 %, DRAM at 55 %, at 44 % of the
+// warps an SM holds and with spills (below).  Latent rows: 8200 tokens with 64
+// heads 27 us, 5.7 TB/s.  All in CUDA graphs; a call from the host takes 7 us.
 #include <cuda_bf16.h>
 #include <math.h>
 
@@ -430,6 +431,9 @@ __device__ __forceinline__ void quantise_rows(const __nv_bfloat16* src, long lon
   }
 }
 
+// Four CTAs per SM leave 64 registers, at which the rotating kernels spill: 48
+// bytes of stores and 24 of loads into the bf16 cache, 56 and 296 (half
+// layout) or 8 and 20 (interleaved) into the 4-bit one.
 template <int MODE, bool KV4>
 __global__ void __launch_bounds__(kThreads, 4)
     kv_append_gqa_kernel(const __grid_constant__ GqaParams p, int group) {
@@ -632,7 +636,8 @@ namespace {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// Warps that run at once (four CTAs of eight on every SM): a call of fewer
+// Warps that run at once on 148 SMs (four CTAs of eight on each; the latent
+// append in the half layout, with 80 registers, has three): a call of fewer
 // tokens spreads each token's heads over as many as fit in that one wave.
 constexpr long long kFillWarps = 148 * 32;
 

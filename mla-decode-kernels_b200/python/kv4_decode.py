@@ -33,8 +33,10 @@ def new_cache(num_blocks, block_size, num_kv_heads, group=64, device="cuda"):
 
 def gqa_decode_kv4(q, k_cache, v_cache, block_table, seq_lens, scale, out=None):
     """out [B, Hq, 128] bf16: softmax_t(q . K[t] * scale) @ V[t] over each
-    request's first seq_lens[b] tokens, 0 for a request without tokens.  Block
-    ids outside the cache set bit 1 of get_status() and read block 0."""
+    request's first seq_lens[b] tokens (at most the block table's row), 0 for a
+    request without tokens; q contiguous.  Block ids outside the cache set bit 1
+    of get_status() and read block 0.  A group of the cache that holds a NaN or
+    an infinity spoils all dims of its request's q heads of that kv head."""
     return _ext.gqa_decode_kv4(q, k_cache, v_cache, block_table, seq_lens, scale, out)
 
 

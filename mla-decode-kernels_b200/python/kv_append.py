@@ -50,10 +50,13 @@ def rope_cos_sin(positions, rotary_dim, base=10000.0, scaling=None, device="cuda
       "bands"   angles with a wavelength under original / high are kept, over
                 original / low divided by factor, linear in between; keys
                 original (trained positions), low (1.0), high (4.0)
-      "yarn"    between f_j / factor and f_j by a ramp over the number of turns
-                that angle j makes in `original` positions, from slow (1.0) to
-                fast (32.0) turns; cosines and sines are multiplied by
-                attention (0.1 ln(factor) + 1)
+      "yarn"    f_j up to the angle that makes fast (32.0) turns in `original`
+                positions, f_j / factor from the one that makes slow (1.0), and
+                linear in j between those two (rounded down and up, as trained
+                models' tables are); cosines and sines are multiplied by
+                attention (0.1 ln(factor) + 1).  The method is Peng et al.,
+                "YaRN: Efficient Context Window Extension of Large Language
+                Models", 2023
     """
     if rotary_dim < 16 or rotary_dim > 128 or rotary_dim % 16:
         raise ValueError("rotary_dim must be a multiple of 16 up to 128")
