@@ -18,7 +18,7 @@
 //     that meets 16 n or a byte loses bits below 2^-13 of that, 2^-21 at most,
 //     one that meets n below 2^-17, 2^-25 at most.  The offset 8 is taken off
 //     by the centres' product, as the centre -8 s times the sum of the rounded
-//     values, so that codes of 8 cancel whatever was rounded.
+//     values, which is what the codes met.
 //   * V: the same four values, again raw; a byte's sum is 16 out' + out, which
 //     the end resolves.  The offset 8 joins the centres, through one product
 //     of the weights with a constant.  The raw sums grow with the context
@@ -28,8 +28,14 @@
 // that meet codes to fp16, 2^-11; the weights p_t that meet centres to bf16,
 // 2^-8, the widest (their range is not fp16's: p_t is 2^9 over a scale); the
 // sums of q that meet centres and -8 s to two bf16 parts, 2^-17; ex2.approx,
-// 2^-22.  Everything else is summed in fp32.  Against 64 bits the output is off
-// by 0.0018-0.0020 (relative rms), of which its own rounding to bf16 is 0.0017.
+// 2^-22.  Sums are fp32, but a tensor-core product lines its terms up by the
+// operands' nominal exponents, and a subnormal's is 2^-14 whatever its value:
+// what lies below 2^-39 of the largest other operand (measured) is dropped from
+// each term.  For 16 tokens or dims that is up to 17 times 2^-15 of one code's
+// step: 2^-11 of a tile's largest p s for an output, and in a score 2^-11 of s
+// times the largest of 16 q for each of its eight products.  Against 64 bits
+// the output is off by 0.0018-0.0020 (relative rms), of which its own rounding
+// to bf16 is 0.0017.
 // A scale that is NaN or infinite spoils all dims of its request's q heads of
 // that kv head (the product with -8 has zeros that meet it); V's scales count
 // in full from 1e-18 to 1e30, smaller ones lose bits in fp16 and from 1e32 on

@@ -9,7 +9,11 @@ output to bf16, 2^-8; the softmax weight that meets V's centre to bf16, 2^-8;
 the weight times V's scale to fp16, 2^-11; q - q' / 16 of the q values at dims
 2 and 6 of every eight to fp16, 2^-11, and a q below 2^-13 of its head's
 largest to a step of 2^-20 of that; the sums of q that meet centres and -8 s to
-two bf16 parts, 2^-17; ex2.approx, 2^-22; fp32 sums.
+two bf16 parts, 2^-17; ex2.approx, 2^-22.  Sums are fp32, except that a product
+of subnormal codes drops what lies below 2^-15 of a code's step, times the
+largest weight and scale of its 16 tokens, from each of 17 terms: with weights
+that differ little within a tile only from the running sum, 2^-21 of a tile's
+share of the bound, else at most 2^-11 of its largest weight times scale.
 """
 
 import pytest

@@ -208,3 +208,46 @@ def test_outputs_that_overlap_between_strides_are_refused():
     kv_append.mla_append(*args, q_pe=full[..., 64:128], out=full[..., 128:])
     assert torch.equal(full[..., 128:], full[..., 64:128])  # no table: a copy
     assert kv_append.get_status(True) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_a_heavy_token_of_zeros_costs_little_of_the_others(group):
+    # One token takes nearly all the weight and its V is 0 (codes 8, centre 0,
+    # scale 1): 8 p s comes and goes in the sums, from which each product may
+    # drop 2^-15 of its tile's largest p s per term, 17 terms.  The other tokens
+    # of V's output, far smaller, are right to that.
+    _, kv4_decode = _modules()
+    S, Hkv, heavy = 176, 2, 70
+    gen = torch.Generator().manual_seed(group)
+    k = 0.1 * torch.randn(S, Hkv, 128, generator=gen)
+    k[heavy, :, 0] = 8.0
+    v = torch.randn(S, Hkv, 128, generator=gen)
+    v[heavy] = 0.0
+    v[heavy, :, 0::group], v[heavy, :, 1::group] = -8.0, 7.0
+    caches = [ref.pack(x.view(S // 16, 1, 16, Hkv, 128).transpose(2, 3), group, value)
+              for x, value in ((k, False), (v, True))]
+    (kn, ks, kc), (vn, vs, vc) = ([t.transpose(2, 3).reshape(S, Hkv, 128) for t in ref.unpack(c, group, value)]
+                                  for c, value in zip(caches, (False, True)))
+    q = 0.05 * torch.randn(1, 8, 128, generator=gen)
+    q[..., 0] = 1.0
+    q = q.bfloat16()
+    table = torch.arange(S // 16, dtype=torch.int32, device="cuda")[None]
+    sl = torch.tensor([S], dtype=torch.int32, device="cuda")
+    got = kv4_decode.gqa_decode_kv4(q.cuda(), *(c.cuda() for c in caches), table, sl, 1.0).cpu().double()[0]
+    assert kv4_decode.get_status(True) == 0
+    a = q.double().view(Hkv, 4, 128)
+    p = torch.softmax(torch.einsum("hgd,thd->hgt", a, kn * ks + kc), -1)
+    assert p[..., heavy].min() > 0.9
+    want = torch.einsum("hgt,thd->hgd", p, vn * vs + vc).reshape(8, 128)
+    bound = torch.einsum("hgt,thd->hgd", p, (vn * vs).abs() + vc.abs()).reshape(8, 128)
+    # a score's error: 2^-11 of the q that meet dims 2 and 6 of eight, 2^-11 of
+    # the largest q per product of 16 dims, eight of them, and 2^-16 for the sums
+    d = torch.zeros_like(a)
+    d[..., 2::4] = 2.0 ** -11 * (a[..., 2::4].abs() + a[..., 3::4].abs() / 16)
+    e = torch.einsum("hgd,thd->hgt", d, (kn * ks).abs()) + 2.0 ** -8 * a.abs().amax(-1, keepdim=True) * ks.amax(-1).T[:, None]
+    e = p * (e + 2.0 ** -16 * torch.einsum("hgd,thd->hgt", a.abs(), 8 * ks + kc.abs()))
+    moved = torch.einsum("hgt,thd->hgd", e, (vn * vs).abs() + vc.abs()).reshape(8, 128) + e.sum(-1).reshape(8, 1) * want.abs()
+    drop = (p[:, :, None] * vs.permute(1, 2, 0)[:, None]).unflatten(-1, (-1, 16)).amax(-1).sum(-1).reshape(8, 128)
+    tol = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -11) * bound + moved + 2.0 ** -11 * drop
+    assert torch.all((got - want).abs() <= tol), ((got - want).abs() / tol).max()
